@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libftnn_hip.so")
 SOURCES = ["ftnn_api.hip", "pack_kernels.hip", "mm_kernels.hip", "mfma_kernels.hip", "rows_kernels.hip", "stem_kernels.hip",
-           "direct_kernels.hip", "ftnn_net.hip", "host_hash.cpp"]   # the last one is plain host C++
+           "direct_kernels.hip", "ftnn_net.hip", "i8_kernels.hip", "kv4_kernels.hip", "ftnn_tokens.hip", "host_hash.cpp"]   # the last one is plain host C++
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -75,6 +75,15 @@ _L.ftnn_host_cached_weight_bytes.restype = C.c_int64
 _L.ftnn_host_hash128.restype = None
 _L.ftnn_host_hash128.argtypes = [_vp, C.c_int64, C.c_int, C.POINTER(C.c_uint64)]
 _L.ftnn_static_scratch_bytes.restype = C.c_int64
+_i64 = C.c_int64
+_L.ftnn_i8_row_bytes.restype = _i64
+_L.ftnn_quantize_rows_i8.argtypes = [C.c_int, _vp, _i64, _i64, C.c_int, _vp, _i64, _vp, _vp]
+_L.ftnn_mm_i8.argtypes = [C.c_int, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, C.c_int, _vp, _i64, _vp]
+_L.ftnn_mm_i8_rows_scratch_bytes.restype = _i64
+_L.ftnn_mm_i8_rows_scratch_bytes.argtypes = [C.c_int, _i64, _i64, C.c_int]
+_L.ftnn_mm_i8_rows.argtypes = [C.c_int, C.c_int, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, C.c_int, _vp, _i64, _vp, _i64, _vp]
+_L.ftnn_kv4_page_bytes.restype = _i64
+_L.ftnn_kv4_page_bytes.argtypes = [C.c_int] * 3
 
 EXPORTS = ("tnns_conv", "tnns_gemm", "t2r_p2_opt", "b2r", "mm_tnn", "mm_tbn", "mm_btn", "mm_bnn",
            "bitpacking2", "ternarize_opt_avx2", "binarize_opt_avx2", "ftnn_host_forget_weights",
@@ -86,7 +95,9 @@ EXPORTS = ("tnns_conv", "tnns_gemm", "t2r_p2_opt", "b2r", "mm_tnn", "mm_tbn", "m
            "ftnn_mm_engine", "ftnn_expand_bytes", "ftnn_expand_rows", "ftnn_mm_expanded",
            "ftnn_conv_scratch_bytes", "ftnn_conv_engine", "ftnn_select_conv_engine",
            "ftnn_conv_static",
-           "ftnn_conv_weights_bytes", "ftnn_conv_prepare_weights", "ftnn_conv_prepared", "ftnn_net_create", "ftnn_net_create_ex", "ftnn_net_destroy", "ftnn_net_output_elems", "ftnn_net_run")
+           "ftnn_conv_weights_bytes", "ftnn_conv_prepare_weights", "ftnn_conv_prepared", "ftnn_net_create", "ftnn_net_create_ex", "ftnn_net_destroy", "ftnn_net_output_elems", "ftnn_net_run",
+           "ftnn_i8_row_bytes", "ftnn_quantize_rows_i8", "ftnn_mm_i8", "ftnn_mm_i8_rows_scratch_bytes", "ftnn_mm_i8_rows",
+           "ftnn_kv4_page_bytes", "ftnn_kv4_append", "ftnn_kv4_read", "ftnn_kv4_attention_scratch_bytes", "ftnn_kv4_attention")
 
 ENGINE_AUTO, ENGINE_VALU, ENGINE_MFMA_I8, ENGINE_MFMA_F4 = 0, 1, 2, 3
 ENGINE_NAMES = {ENGINE_VALU: "valu", ENGINE_MFMA_I8: "mfma_i8", ENGINE_MFMA_F4: "mfma_f4"}
@@ -351,6 +362,221 @@ def pack_gemm_operand(x):
     i, j = x.shape
     out = _empty(max(i * j // 32, 1), "int64", x.device)
     _check(_L.ftnn_pack_gemm_operand(_f32(x), i, j, _dev(out), _stream()))
+    return out
+
+
+# ------------------------------------------------ operators of token models in few bits
+
+F32, F16, BF16 = 0, 1, 2
+
+
+def _dtype(dt):
+    t = torch or _torch()
+    code = F32 if dt is t.float32 else F16 if dt is t.float16 else BF16 if dt is t.bfloat16 else None
+    if code is None:
+        raise FtnnError("expected float32, float16 or bfloat16, got %s" % (dt,))
+    return code
+
+
+def _need(cond, *text):
+    if not cond:
+        raise FtnnError(text[0] % text[1:])
+
+
+def _here(t, name, dtype=None, dims=None, shape=None):
+    """data of a tensor on the current device whose last dimension is contiguous"""
+    _need(t.is_cuda and t.device.index == torch._C._cuda_getDevice(), "%s: expected a tensor on the current GPU", name)
+    _need(dtype is None or t.dtype == dtype, "%s: expected %s, got %s", name, dtype, t.dtype)
+    _need(dims is None or t.dim() == dims, "%s: expected %s dimensions, got %d", name, dims, t.dim())
+    _need(shape is None or t.shape == shape, "%s: expected shape %s, got %s", name, shape, tuple(t.shape))
+    _need(t.dim() == 0 or t.shape[-1] <= 1 or t.stride(-1) == 1, "%s: its last dimension has to be contiguous", name)
+    return t.data_ptr()
+
+
+def _flat(t, name, dtype, shape):
+    p = _here(t, name, dtype, None, shape)
+    _need(t.is_contiguous(), "%s: expected a contiguous tensor", name)
+    return p
+
+
+def _row_stride(t, least):
+    """values between rows; whatever torch says of a single row"""
+    return t.stride(0) if t.shape[0] > 1 else max(least, t.shape[1])
+
+
+def i8_row_bytes(k):
+    """codes of a row of k, with the zeros up to a multiple of 16"""
+    return int(_L.ftnn_i8_row_bytes(k))
+
+
+def quantize_rows_i8(x, q=None, scale=None):
+    """ftnn_quantize_rows_i8: rows of floats [rows][k] -> (8-bit codes [rows][i8_row_bytes(k)], a scale per row)."""
+    t = torch or _torch()
+    xp = _here(x, "x", None, 2)
+    code = _dtype(x.dtype)
+    rows, k = x.shape
+    _need(k > 0, "x: rows of no values")
+    nb = i8_row_bytes(k)
+    if q is None:
+        q = t.empty((rows, nb), dtype=t.int8, device=x.device)
+    if scale is None:
+        scale = t.empty((rows,), dtype=t.float32, device=x.device)
+    qp = _here(q, "q", t.int8, 2)
+    _need(q.shape[0] == rows and q.shape[1] >= nb, "q: expected %d rows of at least %d codes", rows, nb)
+    _check(_L.ftnn_quantize_rows_i8(code, xp, _row_stride(x, k), rows, k, qp, _row_stride(q, nb), _flat(scale, "scale", t.float32, (rows,)), _stream()))
+    return q, scale
+
+
+def _codes(t, name, k):
+    """pointer, stride and number of rows of codes"""
+    p = _here(t, name, torch.int8, 2)
+    nb = (k + 15) // 16 * 16
+    _need(t.shape[1] >= nb, "%s: rows of %d codes, %d are read", name, t.shape[1], nb)
+    return p, _row_stride(t, nb), t.shape[0]
+
+
+def _result(out, m, n, dtype, device):
+    t = torch
+    if out is None:
+        out = t.empty((m, n), dtype=t.float32 if dtype is None else dtype, device=device)
+    _need(dtype is None or out.dtype == dtype, "out: expected %s, got %s", dtype, out.dtype)
+    p = _here(out, "out", None, 2, (m, n))
+    return out, p, _row_stride(out, n), _dtype(out.dtype)
+
+
+def mm_i8(a, a_scale, b, b_scale, k, bias=None, dtype=None, out=None):
+    """ftnn_mm_i8: codes a [m][..] and b [n][..] with a scale per row each -> [m][n], float32 unless dtype or out says otherwise."""
+    t = torch or _torch()
+    _need(k > 0, "rows of %d codes", k)
+    ap, a_stride, m = _codes(a, "a", k)
+    bp, b_stride, n = _codes(b, "b", k)
+    out, op, o_stride, code = _result(out, m, n, dtype, a.device)
+    _check(_L.ftnn_mm_i8(code, ap, a_stride, _flat(a_scale, "a_scale", t.float32, (m,)), bp, b_stride, _flat(b_scale, "b_scale", t.float32, (n,)),
+                         None if bias is None else _flat(bias, "bias", t.float32, (n,)), m, n, k, op, o_stride, _stream()))
+    return out
+
+
+def mm_i8_rows_scratch_bytes(ternary, m, n, k):
+    return int(_L.ftnn_mm_i8_rows_scratch_bytes(int(ternary), m, n, k))
+
+
+def mm_i8_rows(a, a_scale, rows, b_scale, n, k, ternary, bias=None, dtype=None, out=None, scratch=None):
+    """ftnn_mm_i8_rows: codes a [m][..] against n packed rows (pack_weights or pack_gemm_operand) of k lanes -> [m][n]."""
+    t = torch or _torch()
+    _need(k > 0 and n > 0, "%d rows of %d lanes", n, k)
+    ap, a_stride, m = _codes(a, "a", k)
+    rp = _here(rows, "rows", t.int64)
+    _need(rows.is_contiguous() and rows.numel() >= n * row_words(k, 1, 1, ternary), "rows: expected %d packed rows of %d words", n, row_words(k, 1, 1, ternary))
+    out, op, o_stride, code = _result(out, m, n, dtype, a.device)
+    need = mm_i8_rows_scratch_bytes(ternary, m, n, k)
+    if scratch is None and need > 0:
+        scratch = t.empty(need, dtype=t.uint8, device=a.device)
+    sp, sb = (None, 0) if scratch is None else (_here(scratch, "scratch"), scratch.numel() * scratch.element_size())
+    _need(scratch is None or scratch.is_contiguous(), "scratch: expected a contiguous tensor")
+    _check(_L.ftnn_mm_i8_rows(int(ternary), code, ap, a_stride, _flat(a_scale, "a_scale", t.float32, (m,)), rp, _flat(b_scale, "b_scale", t.float32, (n,)),
+                              None if bias is None else _flat(bias, "bias", t.float32, (n,)), m, n, k, op, o_stride, sp, sb, _stream()))
+    return out
+
+
+class Kv4Desc(C.Structure):
+    """ftnn_kv4_t"""
+    _fields_ = [("d_cache", _vp), ("pages", _i64), ("heads", C.c_int), ("dim", C.c_int), ("page", C.c_int), ("sequences", C.c_int),
+                ("tokens", C.c_int), ("width", C.c_int), ("table_stride", _i64), ("d_table", _vp), ("d_lens", _vp), ("d_starts", _vp)]
+
+
+_kvp = C.POINTER(Kv4Desc)
+_L.ftnn_kv4_append.argtypes = [_kvp, C.c_int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _i64, _i64, _vp, _vp]
+_L.ftnn_kv4_read.argtypes = [_kvp, C.c_int, _vp, _vp, _vp]
+_L.ftnn_kv4_attention_scratch_bytes.restype = _i64
+_L.ftnn_kv4_attention_scratch_bytes.argtypes = [_kvp, C.c_int, C.c_int]
+_L.ftnn_kv4_attention.argtypes = [_kvp, C.c_int, C.c_int, _vp, _i64, _i64, C.c_float, C.c_int, _vp, _vp, _i64, _vp]
+
+
+def kv4_page_bytes(heads, dim, page):
+    n = int(_L.ftnn_kv4_page_bytes(heads, dim, page))
+    if n < 0:
+        _check(n)
+    return n
+
+
+def _kv4(cache, table, lens, starts, tokens, heads, dim, page):
+    t = torch or _torch()
+    nb = kv4_page_bytes(heads, dim, page)
+    cp = _here(cache, "cache", t.uint8, 2)
+    _need(cache.is_contiguous() and cache.shape[1] == nb, "cache: expected contiguous pages of %d bytes, got shape %s", nb, tuple(cache.shape))
+    tp = _here(table, "table", t.int32, 2)
+    n, width = table.shape
+    return Kv4Desc(cp, cache.shape[0], heads, dim, page, n, tokens, width, _row_stride(table, width), tp,
+                   _flat(lens, "lens", t.int32, (n,)), _flat(starts, "starts", t.int32, (n + 1,)))
+
+
+def _token_rows(x, name, dtype, tokens, dim):
+    """pointer, strides and heads of [tokens][heads][dim]"""
+    p = _here(x, name, dtype, 3)
+    _need(x.shape[0] == tokens and x.shape[2] == dim, "%s: expected %d tokens of %d channels, got shape %s", name, tokens, dim, tuple(x.shape))
+    return p, x.stride(0), x.stride(1), x.shape[1]
+
+
+def kv4_append(cache, table, lens, starts, k, v, page, q=None, cos=None, sin=None, neighbours=False, q_out=None):
+    """ftnn_kv4_append: keys and values [tokens][heads][dim] of the new tokens into the cache [pages][kv4_page_bytes(...)].  table
+    [sequences][width], lens [sequences] (with the new tokens), starts [sequences + 1]: int32.  Keys are rotated by cos, sin
+    [positions][rot / 2] where given, and queries q with them: returns those, or None."""
+    t = torch or _torch()
+    _need(k.dim() == 3, "k: expected 3 dimensions, got %d", k.dim())
+    tokens, heads, dim = k.shape
+    d = _kv4(cache, table, lens, starts, tokens, heads, dim, page)
+    code = _dtype(k.dtype)
+    kp = _token_rows(k, "k", k.dtype, tokens, dim)
+    vp = _token_rows(v, "v", k.dtype, tokens, dim)
+    _need(vp[3] == heads, "v: expected %d heads, got %d", heads, vp[3])
+    cp = sp = None
+    positions = rot = 0
+    _need((cos is None) == (sin is None), "cos and sin go together")
+    if cos is not None:
+        cp = _here(cos, "cos", t.float32, 2)
+        positions, rot = cos.shape[0], 2 * cos.shape[1]
+        _need(cos.is_contiguous() and rot > 0, "cos: expected contiguous rows")
+        sp = _flat(sin, "sin", t.float32, cos.shape)
+    qp, op = (None, 0, 0, 0), None
+    if q is not None:
+        qp = _token_rows(q, "q", k.dtype, tokens, dim)
+        if q_out is None:
+            q_out = t.empty(q.shape, dtype=q.dtype, device=q.device)
+        op = _flat(q_out, "q_out", k.dtype, q.shape)
+    _need(q is not None or q_out is None, "q_out without q")
+    _check(_L.ftnn_kv4_append(C.byref(d), code, *kp[:3], *vp[:3], cp, sp, positions, rot, int(neighbours), qp[3], *qp[:3], op, _stream()))
+    return q_out
+
+
+def kv4_read(cache, table, lens, starts, tokens, heads, dim, page, dtype=None, k=None, v=None):
+    """ftnn_kv4_read: (keys, values) [tokens][heads][dim] of the last starts[s + 1] - starts[s] tokens of each sequence."""
+    t = torch or _torch()
+    d = _kv4(cache, table, lens, starts, tokens, heads, dim, page)
+    dtype = dtype or (k.dtype if k is not None else v.dtype if v is not None else t.float32)
+    shape = (tokens, heads, dim)
+    k, v = (t.empty(shape, dtype=dtype, device=cache.device) if x is None else x for x in (k, v))
+    _check(_L.ftnn_kv4_read(C.byref(d), _dtype(dtype), _flat(k, "k", dtype, shape), _flat(v, "v", dtype, shape), _stream()))
+    return k, v
+
+
+def kv4_attention(q, cache, table, lens, starts, heads, page, scale=None, max_len=0, out=None, scratch=None):
+    """ftnn_kv4_attention: queries [tokens][heads_q][dim] of the new tokens over what the cache holds of their sequences, each token
+    seeing itself and those before it; scale defaults to dim ** -0.5.  Rows of no sequence are left as they are in out (not set in one
+    that is made here)."""
+    t = torch or _torch()
+    _need(q.dim() == 3, "q: expected 3 dimensions, got %d", q.dim())
+    tokens, heads_q, dim = q.shape
+    d = _kv4(cache, table, lens, starts, tokens, heads, dim, page)
+    qp = _token_rows(q, "q", q.dtype, tokens, dim)
+    if out is None:
+        out = t.empty(q.shape, dtype=q.dtype, device=q.device)
+    op = _flat(out, "out", q.dtype, q.shape)
+    need = int(_L.ftnn_kv4_attention_scratch_bytes(C.byref(d), heads_q, max_len))
+    if scratch is None and need > 0:
+        scratch = t.empty(need, dtype=t.uint8, device=q.device)
+    sp, sb = (None, 0) if scratch is None else (_here(scratch, "scratch"), scratch.numel() * scratch.element_size())
+    _need(scratch is None or scratch.is_contiguous(), "scratch: expected a contiguous tensor")
+    _check(_L.ftnn_kv4_attention(C.byref(d), _dtype(q.dtype), heads_q, *qp[:3], dim ** -0.5 if scale is None else scale, max_len, op, sp, sb, _stream()))
     return out
 
 

@@ -354,6 +354,115 @@ FTNN_API int ftnn_pack_weights(int ternary, const float *d_w, const float *d_thr
  */
 FTNN_API int ftnn_pack_gemm_operand(const float *d_x, int I, int J, int64_t *d_out, void *stream);
 
+/* ------------------------------- 3. operators of token models in few bits (device memory) */
+
+/*
+ * No counterpart in the reference.  Rows of activations as 8-bit codes with a scale each, products of them with 8-bit weights
+ * and with the packed ternary and binary weights of this library, and a paged cache of keys and values in 4-bit codes
+ * with the attention that reads it.  Calls of no rows or tokens do nothing and succeed.
+ */
+
+/* element types of the tensors in floating point */
+#define FTNN_F32 0
+#define FTNN_F16 1
+#define FTNN_BF16 2
+
+/* bytes of a row of K 8-bit codes: K rounded up to a multiple of 16 */
+FTNN_API int64_t ftnn_i8_row_bytes(int K);
+
+/*
+ * Rows of floats -> 8-bit codes, one scale per row:  scale = max |x| / 127,  q = x / scale rounded to the nearest integer, ties
+ * to even, exactly (whatever max |x| is, zero and subnormal numbers included; a row of zeros has scale 0 and codes 0).  A row with a
+ * NaN or an infinity has scale NaN and codes 0, so that what is computed from it is NaN.  d_x: rows of K values, x_stride
+ * values apart, aligned to their type.  d_q: 16-byte aligned rows, q_stride bytes apart (a multiple of 16, at least
+ * ftnn_i8_row_bytes(K)), each written up to ftnn_i8_row_bytes(K) with zeros behind the K-th code.  Activations (a scale per
+ * token) and weights (a scale per channel) alike.
+ */
+FTNN_API int ftnn_quantize_rows_i8(int dtype, const void *d_x, int64_t x_stride, int64_t rows, int K, int8_t *d_q,
+                                   int64_t q_stride, float *d_scale, void *stream);
+
+/*
+ * y[m][n] = sum_k a[m][k] b[n][k] * sa[m] * sb[n] + bias[n], sums in 32-bit integers, scales applied in fp32 in that order, one
+ * rounding to the result's type.  d_a, d_b: rows of 8-bit codes as above (16-byte aligned, strides multiples of 16; the bytes from K up to
+ * ftnn_i8_row_bytes(K) are zero in one of the two).  d_bias may be NULL.  d_y: rows of N values, y_stride values apart.  K at
+ * most 131071 (32-bit sums of any codes); M and N below 2^31, M * N below 2^40.
+ */
+FTNN_API int ftnn_mm_i8(int dtype, const int8_t *d_a, int64_t a_stride, const float *d_sa, const int8_t *d_b,
+                        int64_t b_stride, const float *d_sb, const float *d_bias, int64_t M, int64_t N, int K, void *d_y,
+                        int64_t y_stride, void *stream);
+
+/*
+ * The same with packed weights: d_b holds N rows of ftnn_pack_weights(ternary, ..., KN = N, C = K, 1, 1) or, for K a multiple of
+ * 256, of ftnn_pack_gemm_operand (16-byte aligned).  d_sb: a scale per channel.  The bytes of d_a from K up to ftnn_i8_row_bytes(K) have to be
+ * zero.  d_scratch (16-byte aligned, ftnn_mm_i8_rows_scratch_bytes() bytes, 0 for few tokens) holds the weights as 8-bit codes.
+ */
+FTNN_API int64_t ftnn_mm_i8_rows_scratch_bytes(int ternary, int64_t M, int64_t N, int K);
+FTNN_API int ftnn_mm_i8_rows(int ternary, int dtype, const int8_t *d_a, int64_t a_stride, const float *d_sa,
+                             const int64_t *d_b, const float *d_sb, const float *d_bias, int64_t M, int64_t N, int K,
+                             void *d_y, int64_t y_stride, void *d_scratch, int64_t scratch_bytes, void *stream);
+
+/*
+ * A paged cache of keys and values in 4-bit codes, and the tokens that a call is about.
+ *
+ * The cache is `pages` pages of ftnn_kv4_page_bytes() bytes; a page holds `page` tokens (16, 32, 64, 128 or 256), one block per head
+ * (dim 64, 96, 128 or 256):
+ *   key codes    [page][dim]             4 bits each, the element of the lower index in the lower half of a byte
+ *   value codes  [page / 8][dim][8]      8 tokens of a channel lie together
+ *   keys' (scale, zero), then values'    [page][2] bfloat16
+ * A code c stands for zero + scale * c.
+ *
+ * Token p of sequence s lies in slot p % page of page table[s * table_stride + p / page].  Sequence s holds lens[s] tokens (at most
+ * width * page count), and the last starts[s + 1] - starts[s] of them are the call's: rows starts[s] .. starts[s + 1] - 1 of its
+ * tensors, each with `tokens` rows.  starts[0] is 0 and starts do not fall.  Rows from starts[sequences] on are left as they are.
+ * The arrays are read on the device: no call waits for it.  A page number outside of the cache is no error: its tokens
+ * are not stored, read as zero and are not seen by attention.
+ */
+typedef struct ftnn_kv4 {
+    void *d_cache;          /* 16-byte aligned                              */
+    int64_t pages;          /* pages in the cache                           */
+    int heads, dim, page;   /* heads of keys and values; tokens per page    */
+    int sequences, tokens;  /* sequences; rows of the call's tensors        */
+    int width;              /* pages that a sequence may have               */
+    int64_t table_stride;   /* entries between sequences of the table       */
+    const int32_t *d_table; /* [sequences][width]                           */
+    const int32_t *d_lens;  /* [sequences]                                  */
+    const int32_t *d_starts;/* [sequences + 1]                              */
+} ftnn_kv4_t;
+
+FTNN_API int64_t ftnn_kv4_page_bytes(int heads, int dim, int page);
+
+/*
+ * Appends the call's keys and values [tokens][heads][dim].  Keys are rotated by their position on the way: with cos, sin =
+ * d_cos, d_sin[position][i], i < rot / 2, the pair (x1, x2) becomes (x1 cos - x2 sin, x2 cos + x1 sin), computed in 64 bits and rounded to
+ * fp32; pairs are elements (i, i + rot / 2), or (2 i, 2 i + 1) if `neighbours` is set; elements from rot on stay (rot even, 0: no rotation,
+ * d_cos and d_sin unused).  Then per token and head: zero = the smallest value and scale = (largest - smallest) / 15, both
+ * rounded to bfloat16; code = (x - zero) / scale rounded to the nearest integer, ties to even, kept within 0 .. 15 (0 where scale is 0).
+ * A group with a NaN, an infinity or a spread beyond fp32 gets scale and zero NaN.  With heads_q > 0 the queries d_q
+ * [tokens][heads_q][dim] of the same tokens are rotated into d_q_out, contiguous, in the same launch.  Strides in values; channels are
+ * contiguous.  Tokens whose position is negative or not below `positions` (rows of the tables; not looked at if rot is 0) are not stored, and
+ * their queries not written.  A page that receives tokens in a call belongs to one sequence.
+ */
+FTNN_API int ftnn_kv4_append(const ftnn_kv4_t *kv, int dtype, const void *d_k, int64_t k_token_stride,
+                             int64_t k_head_stride, const void *d_v, int64_t v_token_stride, int64_t v_head_stride,
+                             const float *d_cos, const float *d_sin, int positions, int rot, int neighbours, int heads_q,
+                             const void *d_q, int64_t q_token_stride, int64_t q_head_stride, void *d_q_out, void *stream);
+
+/* what the cache holds of the call's tokens as values: d_k, d_v [tokens][heads][dim], contiguous; either may be NULL */
+FTNN_API int ftnn_kv4_read(const ftnn_kv4_t *kv, int dtype, void *d_k, void *d_v, void *stream);
+
+/*
+ * Attention of the call's queries d_q [tokens][heads_q][dim] over the cache, heads_q a multiple of heads (query head j reads
+ * head j / (heads_q / heads)): softmax(scale q k) v over the tokens up to the query's own.  d_out: [tokens][heads_q][dim],
+ * contiguous, of the queries' type (FTNN_F16 or FTNN_BF16); zeros for a query that sees no token.  max_len: the largest of lens if the
+ * caller knows it, else 0; it decides how the work is split and nothing else.  d_scratch: 16-byte aligned,
+ * ftnn_kv4_attention_scratch_bytes() bytes (0: none needed).  Products are computed in bfloat16 with fp32 sums, queries and
+ * weights of FTNN_F16 as two bfloat16 each.
+ */
+FTNN_API int64_t ftnn_kv4_attention_scratch_bytes(const ftnn_kv4_t *kv, int heads_q, int max_len);
+FTNN_API int ftnn_kv4_attention(const ftnn_kv4_t *kv, int dtype, int heads_q, const void *d_q, int64_t q_token_stride,
+                                int64_t q_head_stride, float scale, int max_len, void *d_out, void *d_scratch,
+                                int64_t scratch_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
