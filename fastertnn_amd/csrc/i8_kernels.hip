@@ -1,6 +1,7 @@
 // Rows of 8-bit codes with a scale each, and their products with 8-bit and with packed ternary or binary weights.
 #include <algorithm>
 
+#include "i8_forms.h"
 #include "tokens_internal.h"
 
 namespace ftnn {
@@ -182,76 +183,149 @@ __device__ __forceinline__ void unpack32(uint32_t s, uint32_t z, uint32_t (&out)
     }
 }
 
-// Few tokens: KS wavefronts split K over one tile of 16 weight rows x 16 MB tokens and meet in LDS.
-template <I8Weights W, typename T, int MB>
+// Few tokens: KS wavefronts split K over one tile of 16 NB weight rows x 16 MB tokens and meet in LDS.  Operands come straight from memory
+// into registers, the next step's while this one is multiplied.
+template <I8Weights W, typename T, int NB, int MB>
 __global__ __launch_bounds__(512) void k_i8_few(I8Product p, uint32_t ntiles) {
-    constexpr int KS = 8;
-    __shared__ int meet[KS][MB][16][17];
+    constexpr int KS = 8, LD = 16 * NB + 4;
+    extern __shared__ __align__(16) int meet[];   // [KS][16 MB][LD]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
-    const int64_t mt = blockIdx.x / ntiles, n0 = (int64_t)(blockIdx.x - mt * ntiles) * 16, m0 = mt * 16 * MB;
+    const int64_t mt = blockIdx.x / ntiles, n0 = (int64_t)(blockIdx.x - mt * ntiles) * 16 * NB, m0 = mt * 16 * MB;
     const int kb = (p.K + 15) & ~15;   // bytes of a row of codes
-    v4i acc[MB];
+    v4i acc[NB][MB];
 #pragma unroll
-    for (int i = 0; i < MB; i++) acc[i] = v4i{0, 0, 0, 0};
+    for (int j = 0; j < NB; j++)
+#pragma unroll
+        for (int i = 0; i < MB; i++) acc[j][i] = v4i{0, 0, 0, 0};
     const int8_t* a[MB];
 #pragma unroll
     for (int i = 0; i < MB; i++) a[i] = p.a + std::min<int64_t>(m0 + i * 16 + r, p.M - 1) * p.a_stride;
-    auto tokens = [&](int i, int k) -> v4i {   // 16 codes from k on; zeros past the row
-        return k < kb ? *reinterpret_cast<const v4i*>(a[i] + k) : v4i{0, 0, 0, 0};
+    auto piece = [&](const int8_t* row, int k) -> v4i {   // 16 codes from k on; zeros past the row
+        return k < kb ? *reinterpret_cast<const v4i*>(row + k) : v4i{0, 0, 0, 0};
     };
-    const int64_t n = std::min<int64_t>(n0 + r, p.N - 1);
+    // of a token: none where the lane has no token of its own, which spares the L1 most of the work for one token
+    auto token_piece = [&](int i, int k) -> v4i { return k < kb && m0 + 16 * i + r < p.M ? *reinterpret_cast<const v4i*>(a[i] + k) : v4i{0, 0, 0, 0}; };
     if constexpr (W == I8Weights::Codes) {
-        const int8_t* const b = static_cast<const int8_t*>(p.b) + n * p.b_stride;
-        for (int k0 = wave * 64; k0 < kb; k0 += KS * 64) {
-            const int k = k0 + 16 * g;
-            const v4i w = k < kb ? *reinterpret_cast<const v4i*>(b + k) : v4i{0, 0, 0, 0};
+        const int8_t* b[NB];
 #pragma unroll
-            for (int i = 0; i < MB; i++) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, tokens(i, k), acc[i], 0, 0, 0);
+        for (int j = 0; j < NB; j++) b[j] = static_cast<const int8_t*>(p.b) + std::min<int64_t>(n0 + j * 16 + r, p.N - 1) * p.b_stride;
+        // a step is 128 codes of a row, a cache line: two multiplies
+        v4i wn[2][NB], tn[2][MB];
+        auto fetch = [&](int k0) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int k = k0 + 64 * u + 16 * g;
+#pragma unroll
+                for (int j = 0; j < NB; j++) wn[u][j] = piece(b[j], k);
+#pragma unroll
+                for (int i = 0; i < MB; i++) tn[u][i] = token_piece(i, k);
+            }
+        };
+        int k0 = wave * 128;
+        if (k0 < kb) fetch(k0);
+        for (; k0 < kb; k0 += KS * 128) {
+            v4i w[2][NB], t[2][MB];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+#pragma unroll
+                for (int j = 0; j < NB; j++) w[u][j] = wn[u][j];
+#pragma unroll
+                for (int i = 0; i < MB; i++) t[u][i] = tn[u][i];
+            }
+            if (k0 + KS * 128 < kb) fetch(k0 + KS * 128);
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int j = 0; j < NB; j++)
+#pragma unroll
+                    for (int i = 0; i < MB; i++) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][j], t[u][i], acc[j][i], 0, 0, 0);
         }
     } else {
         // two groups of four words per step: lane quarter g takes half g % 2 of group g / 2, 128 lanes in 16 bytes of signs (and zeros)
         constexpr bool TERN = W == I8Weights::Ternary;
         const int groups = (p.K + 255) / 256;
-        const v4u* const b = static_cast<const v4u*>(p.b) + n * groups * (TERN ? 4 : 2);
-        for (int q0 = wave * 2; q0 < groups; q0 += KS * 2) {
-            const int q = q0 + (g >> 1), half = g & 1, k0 = q * 256 + half * 128;
+        const v4u* b[NB];
+#pragma unroll
+        for (int j = 0; j < NB; j++) b[j] = static_cast<const v4u*>(p.b) + std::min<int64_t>(n0 + j * 16 + r, p.N - 1) * groups * (TERN ? 4 : 2);
+        v4u sn[NB], zn[NB];
+        auto fetch = [&](int q0) {
+            const int q = q0 + (g >> 1), half = g & 1;
             const bool in = q < groups;
-            const v4u s = in ? b[q * (TERN ? 4 : 2) + half] : v4u{0, 0, 0, 0}, z = TERN && in ? b[q * 4 + 2 + half] : v4u{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                sn[j] = in ? b[j][q * (TERN ? 4 : 2) + half] : v4u{0, 0, 0, 0};
+                zn[j] = TERN && in ? b[j][q * 4 + 2 + half] : v4u{0, 0, 0, 0};
+            }
+        };
+        int q0 = wave * 2;
+        if (q0 < groups) fetch(q0);
+        for (; q0 < groups; q0 += KS * 2) {
+            const int k0 = (q0 + (g >> 1)) * 256 + (g & 1) * 128;
+            v4u s[NB], z[NB];
+#pragma unroll
+            for (int j = 0; j < NB; j++) s[j] = sn[j], z[j] = zn[j];
+            if (q0 + KS * 2 < groups) fetch(q0 + KS * 2);
 #pragma unroll
             for (int d = 0; d < 4; d++) {
-                uint32_t w[8];
-                unpack32<W>(s[d], z[d], w);
-                const v4i w0 = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]}, w1 = {(int)w[4], (int)w[5], (int)w[6], (int)w[7]};
+                v4i e[MB], o[MB];
 #pragma unroll
                 for (int i = 0; i < MB; i++) {
-                    const v4i lo = tokens(i, k0 + 32 * d), hi = tokens(i, k0 + 32 * d + 16);
-                    uint32_t e[4], o[4];
-                    transpose_bytes({(uint32_t)lo[0], (uint32_t)lo[2], (uint32_t)hi[0], (uint32_t)hi[2]}, e);
-                    transpose_bytes({(uint32_t)lo[1], (uint32_t)lo[3], (uint32_t)hi[1], (uint32_t)hi[3]}, o);
-                    acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w0, v4i{(int)e[0], (int)e[1], (int)e[2], (int)e[3]}, acc[i], 0, 0, 0);
-                    acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w1, v4i{(int)o[0], (int)o[1], (int)o[2], (int)o[3]}, acc[i], 0, 0, 0);
+                    const v4i lo = token_piece(i, k0 + 32 * d), hi = token_piece(i, k0 + 32 * d + 16);
+                    uint32_t x[4], y[4];
+                    transpose_bytes({(uint32_t)lo[0], (uint32_t)lo[2], (uint32_t)hi[0], (uint32_t)hi[2]}, x);
+                    transpose_bytes({(uint32_t)lo[1], (uint32_t)lo[3], (uint32_t)hi[1], (uint32_t)hi[3]}, y);
+                    e[i] = v4i{(int)x[0], (int)x[1], (int)x[2], (int)x[3]}, o[i] = v4i{(int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+                }
+#pragma unroll
+                for (int j = 0; j < NB; j++) {
+                    uint32_t w[8];
+                    unpack32<W>(s[j][d], z[j][d], w);
+                    const v4i w0 = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]}, w1 = {(int)w[4], (int)w[5], (int)w[6], (int)w[7]};
+#pragma unroll
+                    for (int i = 0; i < MB; i++) {
+                        acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w0, e[i], acc[j][i], 0, 0, 0);
+                        acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w1, o[i], acc[j][i], 0, 0, 0);
+                    }
                 }
             }
         }
     }
-    // accumulator e of a lane: weight row 4 g + e, token r
+    // accumulator e of a lane: weight row 4 g + e of its block, token r
 #pragma unroll
-    for (int i = 0; i < MB; i++)
+    for (int j = 0; j < NB; j++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) meet[wave][i][r][4 * g + e] = acc[i][e];
+        for (int i = 0; i < MB; i++) *reinterpret_cast<v4i*>(meet + (wave * 16 * MB + 16 * i + r) * LD + 16 * j + 4 * g) = acc[j][i];
     __syncthreads();
-    for (int t = threadIdx.x; t < MB * 256; t += 512) {
-        const int col = t & 15, tok = t >> 4;
+    for (int t = threadIdx.x; t < 256 * MB * NB; t += 512) {
+        const int col = t % (16 * NB), tok = t / (16 * NB);
         int sum = 0;
 #pragma unroll
-        for (int w = 0; w < KS; w++) sum += meet[w][tok >> 4][tok & 15][col];
-        const int64_t m = m0 + tok, nn = n0 + col;
-        if (m < p.M && nn < p.N) {
-            float y = (float)sum * p.sa[m] * p.sb[nn];
-            if (p.bias) y += p.bias[nn];
-            put_result<T>(p.y, m * p.y_stride + nn, y);
+        for (int w = 0; w < KS; w++) sum += meet[(w * 16 * MB + tok) * LD + col];
+        const int64_t m = m0 + tok, n = n0 + col;
+        if (m < p.M && n < p.N) {
+            float y = (float)sum * p.sa[m] * p.sb[n];
+            if (p.bias) y += p.bias[n];
+            put_result<T>(p.y, m * p.y_stride + n, y);
         }
+    }
+}
+
+// packed rows -> rows of codes, 32 lanes per thread
+template <I8Weights W>
+__global__ __launch_bounds__(256) void k_unpack_rows(const uint32_t* __restrict__ B, int64_t N, int K, int8_t* __restrict__ out, int64_t stride) {
+    constexpr bool TERN = W == I8Weights::Ternary;
+    const int64_t per = stride / 32, words = (int64_t)((K + 255) / 256) * (TERN ? 16 : 8);   // of 32 lanes, of a row
+    for (int64_t u = blockIdx.x * 256ll + threadIdx.x; u < N * per; u += gridDim.x * 256ll) {
+        const int64_t row = u / per, i = u - row * per;
+        const uint32_t* const r = B + row * words + (i / 8) * (TERN ? 16 : 8) + i % 8;
+        uint32_t c[8], e[4], o[4];
+        unpack32<W>(r[0], TERN ? r[8] : 0u, c);
+        transpose_bytes({c[0], c[1], c[2], c[3]}, e);
+        transpose_bytes({c[4], c[5], c[6], c[7]}, o);
+        v4u* const d = reinterpret_cast<v4u*>(out + row * stride + i * 32);
+        d[0] = v4u{e[0], o[0], e[1], o[1]};
+        d[1] = v4u{e[2], o[2], e[3], o[3]};
     }
 }
 
@@ -267,28 +341,64 @@ hipError_t launch_quantize_rows_i8(int dtype, const void* d_x, int64_t x_stride,
     });
 }
 
-int64_t mm_i8_rows_scratch(I8Weights, int64_t, int64_t, int) { return 0; }
+// where packed weights lie as codes: rows of whole cache lines
+static int64_t unpacked_stride(int K) { return ((int64_t)K + 127) / 128 * 128; }
 
-hipError_t launch_mm_i8(I8Weights w, int dtype, const I8Product& p, void*, hipStream_t st) {
-    const uint32_t ntiles = (uint32_t)((p.N + 15) / 16);
-    auto go = [&](auto weights) {
-        constexpr I8Weights W = decltype(weights)::value;
-        return with_type(dtype, [&](auto t) {
-            typedef decltype(t) T;
-            auto run = [&](auto mb) {
-                constexpr int MB = decltype(mb)::value;
-                const int64_t tiles = ntiles * ((p.M + 16 * MB - 1) / (16 * MB));
-                if (tiles > 0x7fffffff) return hipErrorInvalidConfiguration;
-                k_i8_few<W, T, MB><<<dim3((unsigned)tiles), dim3(512), 0, st>>>(p, ntiles);
-                return hipGetLastError();
-            };
-            if (p.M <= 16) return run(std::integral_constant<int, 1>{});
-            return run(std::integral_constant<int, 2>{});
-        });
-    };
-    if (w == I8Weights::Codes) return go(std::integral_constant<I8Weights, I8Weights::Codes>{});
-    if (w == I8Weights::Ternary) return go(std::integral_constant<I8Weights, I8Weights::Ternary>{});
-    return go(std::integral_constant<I8Weights, I8Weights::Binary>{});
+// the form without tiles; none (nb 0) where tiles are ahead.  Tiles hold offsets of a row in a tile in 32 bits
+static I8Few few_of(I8Weights w, const I8Product& p) {
+    const bool packed = w != I8Weights::Codes, wide = p.a_stride >= (8 << 20) || p.b_stride >= (8 << 20);
+    const I8Few f = i8_few(packed, p.M, p.N);
+    return f.nb == 0 && wide ? I8Few{1, 2} : f;
+}
+
+int64_t mm_i8_rows_scratch(I8Weights w, int64_t M, int64_t N, int K) {
+    return i8_few(w != I8Weights::Codes, M, N).nb ? 0 : N * unpacked_stride(K);
+}
+
+template <I8Weights W>
+static hipError_t launch_few(I8Few f, int dtype, const I8Product& p, hipStream_t st) {
+    return with_type(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        auto run = [&](auto nb, auto mb) {
+            constexpr int NB = decltype(nb)::value, MB = decltype(mb)::value, bytes = 8 * 16 * MB * (16 * NB + 4) * 4;
+            const int64_t ntiles = (p.N + 16 * NB - 1) / (16 * NB), tiles = ntiles * ((p.M + 16 * MB - 1) / (16 * MB));
+            if (tiles > 0x7fffffff) return hipErrorInvalidConfiguration;
+            auto* const kern = k_i8_few<W, T, NB, MB>;
+            static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            if (set != hipSuccess) return set;
+            kern<<<dim3((unsigned)tiles), dim3(512), bytes, st>>>(p, (uint32_t)ntiles);
+            return hipGetLastError();
+        };
+        using One = std::integral_constant<int, 1>;
+        using Two = std::integral_constant<int, 2>;
+        using Four = std::integral_constant<int, 4>;
+        if (f.nb == 1 && f.mb == 1) return run(One{}, One{});
+        if (f.nb == 2) return run(Two{}, One{});
+        if constexpr (W == I8Weights::Codes) {
+            return run(One{}, Two{});
+        } else {
+            if (f.nb == 1) return run(One{}, Two{});   // rows too far apart for tiles
+            return f.mb == 1 ? run(Four{}, One{}) : f.mb == 2 ? run(Four{}, Two{}) : run(Four{}, Four{});
+        }
+    });
+}
+
+hipError_t launch_mm_i8(I8Weights w, int dtype, const I8Product& p, void* d_scratch, hipStream_t st) {
+    const I8Few f = few_of(w, p);
+    if (f.nb) {
+        if (w == I8Weights::Codes) return launch_few<I8Weights::Codes>(f, dtype, p, st);
+        return w == I8Weights::Ternary ? launch_few<I8Weights::Ternary>(f, dtype, p, st) : launch_few<I8Weights::Binary>(f, dtype, p, st);
+    }
+    I8Product q = p;
+    if (w != I8Weights::Codes) {
+        const int64_t stride = unpacked_stride(p.K), units = p.N * (stride / 32);
+        auto* const kern = w == I8Weights::Ternary ? k_unpack_rows<I8Weights::Ternary> : k_unpack_rows<I8Weights::Binary>;
+        kern<<<dim3((unsigned)std::min<int64_t>((units + 255) / 256, 16384)), dim3(256), 0, st>>>(static_cast<const uint32_t*>(p.b), p.N, p.K, static_cast<int8_t*>(d_scratch), stride);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        q.b = d_scratch, q.b_stride = stride;
+    }
+    return launch_i8_tiles(dtype, q, st);
 }
 
 }  // namespace ftnn

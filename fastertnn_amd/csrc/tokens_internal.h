@@ -38,6 +38,8 @@ struct I8Product {
     int64_t y_stride;
 };
 hipError_t launch_mm_i8(I8Weights w, int dtype, const I8Product& p, void* d_scratch, hipStream_t st);
+// on tiles through LDS (i8_tiles.hip): strides below 8 MiB, weights in codes
+hipError_t launch_i8_tiles(int dtype, const I8Product& p, hipStream_t st);
 int64_t mm_i8_rows_scratch(I8Weights w, int64_t M, int64_t N, int K);
 
 // ---- kv4_kernels.hip ----

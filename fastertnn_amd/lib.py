@@ -383,6 +383,13 @@ def _need(cond, *text):
         raise FtnnError(text[0] % text[1:])
 
 
+def _given(r):
+    """what csrc/py_call.cpp made of a call: its results, or the library's status where that refused"""
+    if type(r) is int:
+        _check(r)
+    return r
+
+
 def _here(t, name, dtype=None, dims=None, shape=None):
     """data of a tensor on the current device whose last dimension is contiguous"""
     _need(t.is_cuda and t.device.index == torch._C._cuda_getDevice(), "%s: expected a tensor on the current GPU", name)
@@ -411,6 +418,9 @@ def i8_row_bytes(k):
 
 def quantize_rows_i8(x, q=None, scale=None):
     """ftnn_quantize_rows_i8: rows of floats [rows][k] -> (8-bit codes [rows][i8_row_bytes(k)], a scale per row)."""
+    r = (_call or _native()).quantize_rows_i8(x, q, scale)
+    if r is not None:
+        return _given(r)
     t = torch or _torch()
     xp = _here(x, "x", None, 2)
     code = _dtype(x.dtype)
@@ -446,6 +456,9 @@ def _result(out, m, n, dtype, device):
 
 def mm_i8(a, a_scale, b, b_scale, k, bias=None, dtype=None, out=None):
     """ftnn_mm_i8: codes a [m][..] and b [n][..] with a scale per row each -> [m][n], float32 unless dtype or out says otherwise."""
+    r = (_call or _native()).mm_i8(a, a_scale, b, b_scale, k, bias, dtype, out)
+    if r is not None:
+        return _given(r)
     t = torch or _torch()
     _need(k > 0, "rows of %d codes", k)
     ap, a_stride, m = _codes(a, "a", k)
@@ -462,6 +475,9 @@ def mm_i8_rows_scratch_bytes(ternary, m, n, k):
 
 def mm_i8_rows(a, a_scale, rows, b_scale, n, k, ternary, bias=None, dtype=None, out=None, scratch=None):
     """ftnn_mm_i8_rows: codes a [m][..] against n packed rows (pack_weights or pack_gemm_operand) of k lanes -> [m][n]."""
+    r = (_call or _native()).mm_i8_rows(a, a_scale, rows, b_scale, k, bias, dtype, out, n, ternary, scratch)
+    if r is not None:
+        return _given(r)
     t = torch or _torch()
     _need(k > 0 and n > 0, "%d rows of %d lanes", n, k)
     ap, a_stride, m = _codes(a, "a", k)
@@ -521,6 +537,9 @@ def kv4_append(cache, table, lens, starts, k, v, page, q=None, cos=None, sin=Non
     """ftnn_kv4_append: keys and values [tokens][heads][dim] of the new tokens into the cache [pages][kv4_page_bytes(...)].  table
     [sequences][width], lens [sequences] (with the new tokens), starts [sequences + 1]: int32.  Keys are rotated by cos, sin
     [positions][rot / 2] where given, and queries q with them: returns those, or None."""
+    r = (_call or _native()).kv4_append(cache, table, lens, starts, k, v, page, q, cos, sin, neighbours, q_out)
+    if r is not None:
+        return _given(r)[0]
     t = torch or _torch()
     _need(k.dim() == 3, "k: expected 3 dimensions, got %d", k.dim())
     tokens, heads, dim = k.shape
@@ -550,6 +569,9 @@ def kv4_append(cache, table, lens, starts, k, v, page, q=None, cos=None, sin=Non
 
 def kv4_read(cache, table, lens, starts, tokens, heads, dim, page, dtype=None, k=None, v=None):
     """ftnn_kv4_read: (keys, values) [tokens][heads][dim] of the last starts[s + 1] - starts[s] tokens of each sequence."""
+    r = (_call or _native()).kv4_read(cache, table, lens, starts, tokens, heads, dim, page, dtype) if k is None and v is None else None
+    if r is not None:
+        return _given(r)
     t = torch or _torch()
     d = _kv4(cache, table, lens, starts, tokens, heads, dim, page)
     dtype = dtype or (k.dtype if k is not None else v.dtype if v is not None else t.float32)
@@ -563,6 +585,9 @@ def kv4_attention(q, cache, table, lens, starts, heads, page, scale=None, max_le
     """ftnn_kv4_attention: queries [tokens][heads_q][dim] of the new tokens over what the cache holds of their sequences, each token
     seeing itself and those before it; scale defaults to dim ** -0.5.  Rows of no sequence are left as they are in out (not set in one
     that is made here)."""
+    r = (_call or _native()).kv4_attention(cache, table, lens, starts, q, heads, page, q.shape[-1] ** -0.5 if scale is None else scale, max_len, out, scratch)
+    if r is not None:
+        return _given(r)
     t = torch or _torch()
     _need(q.dim() == 3, "q: expected 3 dimensions, got %d", q.dim())
     tokens, heads_q, dim = q.shape

@@ -5,6 +5,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import fastertnn_amd.lib as lib
+from tests import i8_shapes
 from tests import tokens_oracle as ref
 
 pytestmark = pytest.mark.gpu
@@ -119,6 +120,16 @@ def test_product_of_the_largest_sums():
         _check_product(y, a, sa, b, sb, None, k)
 
 
+@pytest.mark.parametrize("m,n,k", [(m, n, k) for (m, n), ks in i8_shapes.TILES.values() for k in ks] + [(*s, k) for s in i8_shapes.FEW_CODES.values() for k in (16, 1025, 3000)])
+def test_product_of_codes_in_each_form(m, n, k):
+    a, sa = _codes(m + n + k, m, k)
+    b, sb = _codes(m * n + k, n, k)
+    bias = _rand(k, (n,))
+    for t, bb in ((torch.float32, bias), (torch.bfloat16, None)):
+        y = lib.mm_i8(a.cuda(), sa.cuda(), b.cuda(), sb.cuda(), k, bias=None if bb is None else bb.cuda(), dtype=t)
+        _check_product(y, a, sa, b, sb, bb, k)
+
+
 @pytest.mark.parametrize("m", [3, 40, 200])
 def test_product_with_strides(m):
     """rows apart, a result inside of a larger tensor, and bytes behind the K-th code of one operand that are not zero"""
@@ -151,6 +162,26 @@ def test_product_with_packed_rows(m, n, k, ternary):
     for t, bb in ((torch.float32, None), (torch.bfloat16, bias), (torch.float16, bias)):
         y = lib.mm_i8_rows(a.cuda(), sa.cuda(), rows, sb.cuda(), n, k, ternary, bias=None if bb is None else bb.cuda(), dtype=t)
         _check_product(y, a, sa, w, sb, bb, k)
+
+
+@pytest.mark.parametrize("ternary", [True, False])
+@pytest.mark.parametrize("m,n,k", [(m, n, ks[-1]) for (m, n), ks in i8_shapes.TILES.values()] + [(*s, k) for s in i8_shapes.FEW_PACKED.values() for k in (16, 1025, 5000)])
+def test_product_with_packed_rows_in_each_form(m, n, k, ternary):
+    a, sa = _codes(m + n + k, m, k)
+    w = ref.lanes(n, k, ternary, torch.Generator().manual_seed(n * k))
+    sb = torch.rand(n) * 0.1 + 0.01
+    y = lib.mm_i8_rows(a.cuda(), sa.cuda(), _packed(w, ternary), sb.cuda(), n, k, ternary)
+    _check_product(y, a, sa, w, sb, None, k)
+
+
+def test_product_of_rows_far_apart():
+    """strides beyond what tiles take"""
+    k, m, n = 100, 90, 9000
+    a, sa = _codes(1, m, k)
+    b, sb = _codes(2, n, k)
+    far = torch.zeros((m, 9 << 20), dtype=torch.int8, device="cuda")
+    far[:, :112] = a.cuda()
+    _check_product(lib.mm_i8(far, sa.cuda(), b.cuda(), sb.cuda(), k), a, sa, b, sb, None, k)
 
 
 @pytest.mark.parametrize("m", [2, 300])

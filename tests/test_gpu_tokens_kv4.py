@@ -357,3 +357,46 @@ def test_refusals():
     assert torch.equal(cache.cpu(), raw)
     none = lib.kv4_attention(q[:0], *a, 2, 16)
     assert none.shape == (0, 4, 64)
+
+
+def test_both_ways_into_the_library(monkeypatch):
+    """the calls through csrc/py_call.cpp give what those through ctypes give, take what they are given, and leave the rest to ctypes"""
+    heads, group, dim, page = 2, 2, 64, 16
+    raw, table, ln, st, n = _setup(30, heads, dim, page, [50, 33], [4, 9])
+    cos, sin, dt, dl, ds = _cuda(*_tables(50, 32), table, ln, st)
+    g = _gen(31)
+    k, v, q = (torch.randn((n, h, dim), generator=g).bfloat16().cuda() for h in (heads, heads, heads * group))
+    x, w, bias = torch.randn((7, 100), generator=g).cuda(), torch.randn((200, 100), generator=g).cuda(), torch.randn(200, generator=g).cuda()
+    lanes = lib.pack_weights(torch.randint(-1, 2, (200, 100, 1, 1), generator=g).float().cuda(), torch.full((200,), 0.5, device="cuda"), True)
+    scratch = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+
+    def calls(yes=True):   # yes: 1 where the plain form is left
+        out = []
+        c = raw.cuda()
+        out += [*lib.quantize_rows_i8(x)]
+        b = lib.quantize_rows_i8(w)
+        out += [lib.mm_i8(*out[:2], *b, 100), lib.mm_i8(*out[:2], *b, 100, bias=bias, dtype=torch.bfloat16), lib.mm_i8(*out[:2], *b, 100, out=torch.empty((7, 200), device="cuda").half())]
+        out += [lib.mm_i8_rows(*out[:2], lanes, b[1], 200, 100, yes), lib.mm_i8_rows(*out[:2], lanes, b[1], 200, 100, yes, bias=bias, dtype=torch.float16, scratch=scratch)]
+        lib.kv4_append(c, dt, dl, ds, k, v, page)
+        out += [c.clone(), lib.kv4_append(c, dt, dl, ds, k, v, page, q=q, cos=cos, sin=sin, neighbours=yes), c]
+        out += [*lib.kv4_read(c, dt, dl, ds, n, heads, dim, page, dtype=torch.float16), lib.kv4_attention(q, c, dt, dl, ds, heads, page),
+                lib.kv4_attention(q, c, dt, dl, ds, heads, page, scale=0.2, max_len=9000, out=torch.empty_like(q), scratch=scratch)]
+        return out
+
+    native, answered = lib._native(), []
+
+    class Spy:
+        def __getattr__(self, name):
+            def fn(*args):
+                r = getattr(native, name)(*args)
+                answered.append(r is not None)
+                return r
+            return fn
+
+    monkeypatch.setattr(lib, "_call", Spy())
+    fast = calls()
+    assert len(answered) == 12 and all(answered)
+    same = lambda a, b: all(torch.equal(s, t) and s.dtype == t.dtype for s, t in zip(a, b))
+    assert same(fast, calls(1))
+    monkeypatch.setattr(lib, "_call", lib._ThroughCtypes())
+    assert same(fast, calls())
