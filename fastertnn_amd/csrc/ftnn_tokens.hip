@@ -39,6 +39,7 @@ int check_kv(const ftnn_kv4_t* kv) {
     if (kv->heads <= 0 || ftnn_kv4_page_bytes(kv->heads, kv->dim, kv->page) < 0)
         return fail(FTNN_EINVAL, "heads %d, dim %d, page %d: dim is 64, 96, 128 or 256, page 16, 32, 64, 128 or 256", kv->heads, kv->dim, kv->page);
     if (kv->sequences < 0 || kv->tokens < 0 || kv->width <= 0 || kv->pages <= 0 || kv->pages > INT32_MAX) return fail(FTNN_EINVAL, "non-positive dimension");
+    if ((int64_t)kv->width * kv->page > 1 << 30) return fail(FTNN_EINVAL, "sequences of more than 2^30 tokens");
     if (kv->heads > 32767) return fail(FTNN_EINVAL, "more than 32767 heads");
     if (kv->table_stride < kv->width) return fail(FTNN_EINVAL, "rows of the table overlap");
     if (!kv->tokens || !kv->sequences) return FTNN_OK;

@@ -248,42 +248,57 @@ __global__ __launch_bounds__(64) void k_kv4_read(Kv4 kv, T* K, T* V) {
 
 // ---------------------------------------------------------------------------------------------------------- attention
 //
-// Scores and outputs come from v_mfma_f32_16x16x32_bf16 on the codes themselves: 128 + code is a bfloat16 whose lowest mantissa bits
-// are the code, so two codes become an operand word with an AND and an OR, and a scale and a zero per token make
-//     q . k_t = ks_t (sum_d q_d (128 + c_td) - 128 sum_d q_d) + kz_t sum_d q_d
-//     sum_t p_t v_td = sum_t w_t (128 + c_td) - 136 sum_t w_t + sum_t p_t (vz_t + 8 vs_t),   w_t = p_t vs_t
-// with w_t rounded to bfloat16 (of FTNN_F16: the sum of two) in both of its sums, so that its rounding only meets code - 8, which is
-// what is rounded where values are multiplied.  The cancelled 128 costs 2^-24 * 128 of a code, far below that.
+// Scores and outputs come from v_mfma_f32_16x16x32_f16 on the codes themselves.  A float16 whose bits are a code c is the subnormal number
+// c 2^-24, and c << 4 is c 2^-20: two codes become an operand word with one AND, four with one shift more.  The factor of 16 at every
+// other element goes into the other operand.  A scale and a zero per token make
+//     q . k_t = ks_t sum_d q_d c_td + kz_t sum_d q_d
+//     sum_t p_t v_td = sum_t w_t c_td - 8 sum_t w_t + sum_t p_t (vz_t + 8 vs_t),   w_t = p_t vs_t
+// with w_t rounded to float16 (where the result is float16: the sum of two) in both of its sums, so that its rounding only meets code - 8,
+// which is what is rounded where values are multiplied.  Queries are scaled by a power of two so that their largest
+// magnitude is in [2^14, 2^15): a float16 or bfloat16 keeps all of its bits, down to 2^-38 of the largest.  Weights are scaled by a power of
+// two that follows the largest vs so far, to at most 2^13 and 2^5 where the largest score so far is their measure: what is below 2^-25 of that is lost.
 //
 // A step is 32 tokens of one wavefront.  Keys are the A operand: row r of block b (two blocks of 16) is token 8 (r / 4) + 4 b + r % 4, so that
 // lane quarter g ends with the scores of tokens 8 g .. 8 g + 7 of its column (a query), in the order in which the second product takes
 // its weights as B operand: no lanes are exchanged.  The values of 8 tokens of a channel are one word of the cache, its A operand.
 // Rows of a tile are (token, query head of the group) pairs of one sequence and one head of keys.
 
-__device__ __forceinline__ v8bf codes8(uint32_t w) {
-    v4u r;
-#pragma unroll
-    for (int p = 0; p < 4; p++) r[p] = (w >> (4 * p) & 0x000F000Fu) | 0x43004300u;
-    return __builtin_bit_cast(v8bf, r);
-}
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    return (uint32_t)__builtin_bit_cast(unsigned short, (__bf16)a) | (uint32_t)__builtin_bit_cast(unsigned short, (__bf16)b) << 16;
-}
-__device__ __forceinline__ float bf16_low(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
-__device__ __forceinline__ float bf16_high(uint32_t w) { return __builtin_bit_cast(float, w & 0xFFFF0000u); }
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 
-// eight values as operand words: word p holds elements p and p + 4, as codes8 has them; the rest in `low` where PARTS is 2
-template <int PARTS>
-__device__ __forceinline__ void split8(const float (&x)[8], v8bf& high, v8bf& low) {
-    v4u h, l;
-#pragma unroll
-    for (int p = 0; p < 4; p++) {
-        h[p] = pack_bf16(x[p], x[p + 4]);
-        if (PARTS == 2) l[p] = pack_bf16(x[p] - bf16_low(h[p]), x[p + 4] - bf16_high(h[p]));
-    }
-    high = __builtin_bit_cast(v8bf, h);
-    if (PARTS == 2) low = __builtin_bit_cast(v8bf, l);
+// eight codes as operand words: word p holds elements p and p + 4, at 2^-24 for even p and 2^-20 for odd p
+__device__ __forceinline__ v8h codes8(uint32_t w) {
+    const uint32_t u = w >> 8;
+    const v4u r = {w & 0x000F000Fu, w & 0x00F000F0u, u & 0x000F000Fu, u & 0x00F000F0u};
+    return __builtin_bit_cast(v8h, r);
 }
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    const v2f f = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, v2h));
+}
+__device__ __forceinline__ v2f unpack_f16(uint32_t w) { return __builtin_convertvector(__builtin_bit_cast(v2h, w), v2f); }
+
+// the other lane quarters' values meet: fn(lanes' own and the 16 and then the 32 lanes across), the same in all quarters, without LDS
+template <typename F>
+__device__ __forceinline__ float over_quarters(float x, F&& fn) {
+    const uint32_t a = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    const uint32_t b = __builtin_bit_cast(uint32_t, fn(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1])));
+    const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fn(__builtin_bit_cast(float, (uint32_t)q[0]), __builtin_bit_cast(float, (uint32_t)q[1]));
+}
+__device__ __forceinline__ float max_over_quarters(float x) {
+    return over_quarters(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float sum_over_quarters(float x) {
+    return over_quarters(x, [](float a, float b) { return a + b; });
+}
+
+// a power of two from its biased exponent
+__device__ __forceinline__ float power(int e) { return __builtin_bit_cast(float, (uint32_t)e << 23); }
+
+constexpr int kMostSplits = 64;
 
 struct Kv4Attend {
     Kv4 kv;
@@ -291,19 +306,20 @@ struct Kv4Attend {
     int heads_q, group, splits;
     float scale2;      // scale * log2(e)
     void* out;
-    float* part;       // [splits][tokens * heads_q][dim], then [splits][tokens * heads_q][2]: sums, maximum and sum of weights
+    float* part;       // [splits][tokens * heads_q][dim], then [splits][tokens * heads_q][2]: sums, maximum (in powers of two) and sum of weights
 };
 
-constexpr int kTile = 16;   // rows of a tile
-
-// which tile of which sequence a workgroup's number is; false behind the last
-__device__ __forceinline__ bool find_tile(const Kv4& kv, int group, int number, int* s, int* tile) {
+// which tile of which sequence a workgroup's number is, with that sequence's rows of the call and its length; false behind the last
+struct Kv4Tile {
+    int s, tile, first, end, length, after;   // after: starts[s + 1]
+};
+__device__ __forceinline__ bool find_tile(const Kv4& kv, int group, int tile_rows, int number, Kv4Tile* t) {
     int before = 0;
     for (int b0 = 0; b0 < kv.sequences; b0 += 64) {
-        const int b = b0 + lane_id();
-        int64_t rows = 0;
-        if (b < kv.sequences) rows = (int64_t)max(0, min(kv.starts[b + 1], kv.tokens) - max(kv.starts[b], 0)) * group;
-        const int tiles = (int)((rows + kTile - 1) / kTile);
+        const int b = min(b0 + lane_id(), kv.sequences - 1);
+        const int from = kv.starts[b], to = kv.starts[b + 1], length = kv.lens[b], first = max(from, 0), end = min(to, kv.tokens);   // together: one wait
+        const int64_t rows = b0 + lane_id() < kv.sequences ? (int64_t)max(0, end - first) * group : 0;
+        const int tiles = (int)((uint32_t)(rows + tile_rows - 1) / (uint32_t)tile_rows);   // (below 2^31 rows in a call)
         int sum = tiles;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -312,188 +328,413 @@ __device__ __forceinline__ bool find_tile(const Kv4& kv, int group, int number, 
         }
         const uint64_t past = __ballot(before + sum > number);
         if (past) {
-            const int l = __ffsll((unsigned long long)past) - 1;
-            *s = b0 + l;
-            *tile = number - before - (__shfl(sum, l) - __shfl(tiles, l));
+            const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)past) - 1);
+            auto at = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            *t = {b0 + l, at(sum) - 1 - (number - before), at(first), at(end), at(length), at(to)};   // the last tiles, which see most, first
             return true;
         }
-        before += __shfl(sum, 63);
+        before += __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(256) void k_kv4_attend(Kv4Attend p) {
-    constexpr int PARTS = std::is_same<T, _Float16>::value ? 2 : 1, ND = D / 32, NB = D / 16, WAVES = 4;
-    extern __shared__ float lds[];   // [WAVES][16][D + 4] sums, then [WAVES][16][2]
+// One sequence and head of the cache as the steps read it.  A lane each holds 64 entries of the table at a time, so that no step waits for an entry before
+// it can ask for its codes (two prompts of 2500 tokens, 4 x 8 heads of 128, 680 -> 597 us).  Positions and offsets in a page are 32 bits, pages are
+// found in 64.
+struct Kv4Pages {
+    const int32_t* table;
+    const char* cache;     // of the head
+    uint32_t page_bytes;
+    int pages, width, shift, mask;   // mask: page - 1
+    int window = 0, ids;             // ids: entry window + lane, -1 outside of the cache
+
+    __device__ __forceinline__ void look(int i) {
+        window = i;
+        const int at = window + lane_id(), id = table[min(at, width - 1)];
+        ids = at < width && (uint32_t)id < (uint32_t)pages ? id : -1;
+    }
+    __device__ __forceinline__ int id(int i) {   // i the same in all lanes, not falling
+        if (i - window >= 64) look(i);
+        return __builtin_amdgcn_readlane(ids, i - window);
+    }
+    __device__ __forceinline__ const char* page(int id) const { return cache + (uint64_t)(uint32_t)max(id, 0) * page_bytes; }
+    // whether entries first .. last are all pages of the cache
+    __device__ __forceinline__ bool all_there(int first, int last) const {
+        bool good = last < width && (window > first || window + lane_id() > last || ids >= 0);
+        for (int i = window > first ? first : window + 64; i <= last; i += 64) {
+            const int id = table[min(min(i + lane_id(), last), width - 1)];
+            good &= (uint32_t)id < (uint32_t)pages;
+        }
+        return __all(good);
+    }
+};
+// where a step's tokens lie: two pages where those hold 16
+struct Kv4Place {
+    const char *first, *second;
+    bool first_there, second_there;
+    __device__ __forceinline__ const char* of(int eight) const { return eight >> 1 ? second : first; }   // the page of tokens 8 eight ..
+};
+__device__ __forceinline__ Kv4Place place_of(Kv4Pages& q, int t0) {
+    const int i = t0 >> q.shift, a = q.id(i), b = q.shift >= 5 ? a : q.id(i + 1);
+    return {q.page(a), q.page(b), a >= 0, b >= 0};
+}
+
+// what a step of 32 tokens takes from the cache
+template <int D>
+struct Kv4Step {
+    uint32_t kw[2][D / 32], vw[D / 16], kp[8], vp[8];
+    bool there;   // the page of the lane's tokens 8 g .. 8 g + 7
+
+    __device__ __forceinline__ void fetch_keys(const Kv4Pages& q, const Kv4Place& p, int t0, int c, int g) {
+        // codes: this lane's row of each block; (scale, zero): tokens 8 g .. 8 g + 7
+        const int kt = t0 + 8 * (c >> 2) + (c & 3), pt = t0 + 8 * g;   // + 4 for the second block
+        const char* const kb = p.of(c >> 2) + (uint32_t)((kt & q.mask) * (D / 2) + g * (D / 8));
+        const char* const pb = p.of(g) + (uint32_t)((q.mask + 1) * D + (pt & q.mask) * 4);
+        __builtin_memcpy(kw[0], __builtin_assume_aligned(kb, 4), D / 8);
+        __builtin_memcpy(kw[1], __builtin_assume_aligned(kb + 4 * (D / 2), 4), D / 8);
+        __builtin_memcpy(kp, __builtin_assume_aligned(pb, 16), 32);
+    }
+    __device__ __forceinline__ void fetch_values(const Kv4Pages& q, const Kv4Place& p, int t0, int c, int g) {
+        const int slot = (t0 + 8 * g) & q.mask;
+        there = g >> 1 ? p.second_there : p.first_there;
+        const char* const b = p.of(g);
+        __builtin_memcpy(vw, __builtin_assume_aligned(b + (uint32_t)((q.mask + 1) * (D / 2) + (slot / 8 * D + c * (D / 16)) * 4), 8), D / 4);
+        __builtin_memcpy(vp, __builtin_assume_aligned(b + (uint32_t)((q.mask + 1) * (D + 4) + slot * 4), 16), 32);
+    }
+};
+
+// CB blocks of 16 rows per wavefront.  WT = 4: the wavefronts of a workgroup split the tokens of one tile and meet in LDS; WT = 1: they have tiles of
+// their own side by side.
+template <typename T, int D, int CB, int WT>
+__global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT, D * CB <= 256 && D < 256 ? 2 : 1) void k_kv4_attend(Kv4Attend p) {
+    constexpr int PARTS = std::is_same<T, _Float16>::value ? 2 : 1, ND = D / 32, NB = D / 16, TILE = 16 * CB, WG_ROWS = WT == 1 ? TILE * 4 : TILE;
+    extern __shared__ __align__(16) float lds[];   // WT = 4: [4][16 CB][D + 4] sums, then [4][16 CB][2]; WT = 1: the wavefronts' queries as operands, [4][CB][ND][64] of 16 bytes
     const Kv4& kv = p.kv;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
-    int s, tile;
-    if (!find_tile(kv, p.group, blockIdx.x, &s, &tile)) return;
-    s = __builtin_amdgcn_readfirstlane(s), tile = __builtin_amdgcn_readfirstlane(tile);
+    Kv4Tile found;
+    if (!find_tile(kv, p.group, WG_ROWS, blockIdx.x, &found)) return;   // (the whole workgroup)
+    const int s = found.s, tile = found.tile;
     const int head = blockIdx.y, split = blockIdx.z;
-    const int first = max(kv.starts[s], 0), end = min(kv.starts[s + 1], kv.tokens), n = end - first;
-    const int64_t held = min((int64_t)max(kv.lens[s], 0), (int64_t)kv.width << kv.shift);
-    // row: token j of the call's n, query head of the group
-    const int64_t row = (int64_t)tile * kTile + c, rows = (int64_t)n * p.group;
-    const bool live = row < rows;
-    const int j = live ? (int)(row / p.group) : n - 1, hq = head * p.group + (live ? (int)(row % p.group) : 0);
-    const int64_t base = (int64_t)kv.lens[s] - kv.starts[s + 1] + first;   // position of token 0
-    const int64_t seen = max((int64_t)0, min(held, base + j + 1));         // tokens that the row sees
-    const int64_t last_row = min((int64_t)tile * kTile + kTile, rows) - 1;
-    const int64_t most = max((int64_t)0, min(held, base + last_row / p.group + 1)), least = max((int64_t)0, min(held, base + (int64_t)tile * kTile / p.group + 1));
-    // queries: word j of a lane's D / 4 channels 8 words apart per quarter
-    v8bf qh[ND], ql[PARTS == 2 ? ND : 1];
-    float qsum = 0.0f;
-    const T* const q = static_cast<const T*>(p.q.p) + (int64_t)(first + j) * p.q.token_stride + (int64_t)hq * p.q.head_stride + g * (D / 4);
+    const int first = found.first, n = found.end - first;
+    const int held = min(max(found.length, 0), kv.width << kv.shift);   // (at most 2^30 tokens, by the host's check)
+    const uint32_t rows = (uint32_t)n * p.group, group = p.group;   // (a call has fewer than 2^31 query rows)
+    const int64_t base = (int64_t)found.length - found.after + first;   // position of the call's first token
+    const uint32_t row0 = (uint32_t)tile * WG_ROWS + (WT == 1 ? wave * TILE : 0);
+    if (WT == 1 && row0 >= rows) return;
+    const uint32_t last_row = min(row0 + TILE, rows) - 1;
+    const int most = (int)max((int64_t)0, min((int64_t)held, base + last_row / group + 1)), least = (int)max((int64_t)0, min((int64_t)held, base + row0 / group + 1));
+    const int steps = (most + 31) / 32, per = (steps + p.splits - 1) / p.splits, from = per * split, to = min(steps, from + per);
+    Kv4Pages seq = {kv.table + s * kv.table_stride, kv.cache + head * kv.head_bytes, (uint32_t)kv.page_bytes, (int)kv.pages, kv.width, kv.shift, kv.page - 1};
+    seq.look((from * 32) >> kv.shift);
+    // the first codes are asked for ahead of the queries.  Of few rows memory is what counts: the codes of the next steps are on their way while one is
+    // computed; of many, the next step's keys when this one's scores are there, its values when this one's sums are
+    constexpr int AHEAD = WT == 1 ? 1 : D <= 128 ? 3 : 2;
+    Kv4Step<D> ring[AHEAD];
+    int st = from + (WT == 1 ? 0 : wave);
+    auto fetch = [&](Kv4Step<D>& x, int step) {
+        const Kv4Place at = place_of(seq, step * 32);
+        x.fetch_keys(seq, at, step * 32, c, g), x.fetch_values(seq, at, step * 32, c, g);
+    };
 #pragma unroll
-    for (int i = 0; i < ND; i++) {
-        float x[8];
-        load8(q + 8 * i, x);
+    for (int i = 0; i < AHEAD; i++)
+        if (st + i * WT < to) fetch(ring[i], st + i * WT);
+    // rows: (token, query head of the group); what a row sees: tokens before `seen`
+    int seen[CB];
+    constexpr bool KEPT = WT > 1;   // queries stay in registers; of many rows they lie in LDS: with them two wavefronts per SIMD do not fit (597 -> 500 us)
+    v8h q[KEPT ? CB : 1][KEPT ? ND : 1];
+    v4u* const mine_q = reinterpret_cast<v4u*>(lds) + (size_t)wave * CB * ND * 64 + lane;
+    float qsum[CB], unit[CB];   // sum of the scaled queries in units of the products; powers of two per unit of score
 #pragma unroll
-        for (int e = 0; e < 8; e++) qsum += x[e];
-        split8<PARTS>(x, qh[i], ql[PARTS == 2 ? i : 0]);
-    }
-    qsum += __shfl_xor(qsum, 16);
-    qsum += __shfl_xor(qsum, 32);
-    v4f o[NB], wsum = {0, 0, 0, 0};
+    for (int b = 0; b < CB; b++) {
+        const uint32_t row = min(row0 + 16 * b + c, rows - 1);
+        const int j = (int)(row / group), hq = head * p.group + (int)(row % group);
+        seen[b] = (int)max((int64_t)0, min((int64_t)held, base + j + 1));
+        const T* const from = static_cast<const T*>(p.q.p) + (int64_t)(first + j) * p.q.token_stride + (int64_t)hq * p.q.head_stride + g * (D / 4);
+        float x[ND][8], top = 0.0f, sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NB; i++) o[i] = v4f{0, 0, 0, 0};
-    float m = -__builtin_inff(), l = 0.0f, zsum = 0.0f;
-    const v4u ones_w = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
-    const v8bf ones = __builtin_bit_cast(v8bf, ones_w);
-
-    const int64_t steps = (most + 31) / 32, per = (steps + p.splits - 1) / p.splits, from = per * split, to = min(steps, from + per);
-    for (int64_t st = from + wave; st < to; st += WAVES) {
-        const int64_t t0 = st * 32;
-        // keys: this lane's row of each block; (scale, zero) and values: tokens 8 g .. 8 g + 7
-        uint32_t kw[2][ND], vw[NB], kp[8], vp[8];
-        bool there;
-        {
-            const int64_t kt = t0 + 8 * (c >> 2) + (c & 3);   // + 4 b
-            const int64_t id = kv.page_of(s, kt);
-            const char* const b = kv.block(max(id, (int64_t)0), head) + (kt & (kv.page - 1)) * (D / 2) + g * (D / 8);
-            __builtin_memcpy(kw[0], __builtin_assume_aligned(b, 4), 4 * ND);
-            __builtin_memcpy(kw[1], __builtin_assume_aligned(b + 4 * (D / 2), 4), 4 * ND);
+        for (int i = 0; i < ND; i++) {
+            load8(from + 8 * i, x[i]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[i][e])), sum += x[i][e];
         }
-        {
-            const int64_t vt = t0 + 8 * g, id = kv.page_of(s, vt), slot = vt & (kv.page - 1);
-            there = id >= 0;
-            const char* const b = kv.block(max(id, (int64_t)0), head);
-            __builtin_memcpy(vw, __builtin_assume_aligned(b + kv.values() + ((slot / 8) * D + c * NB) * 4, 8), 4 * NB);
-            __builtin_memcpy(kp, __builtin_assume_aligned(b + kv.key_params() + slot * 4, 16), 32);
-            __builtin_memcpy(vp, __builtin_assume_aligned(b + kv.value_params() + slot * 4, 16), 32);
-        }
-        float sc[8];
+        top = max_over_quarters(top), sum = sum_over_quarters(sum);
+        const int up = 141 - min(max((int)(__builtin_bit_cast(uint32_t, top) >> 23), 27), 254);   // times 2^up the largest is in [2^14, 2^15)
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
-            v4f a = {-128.0f * qsum, -128.0f * qsum, -128.0f * qsum, -128.0f * qsum};
+        for (int i = 0; i < ND; i++) {
+            v4u h;
 #pragma unroll
-            for (int i = 0; i < ND; i++) {
-                const v8bf k = codes8(kw[b][i]);
-                a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qh[i], a, 0, 0, 0);
-                if (PARTS == 2) a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, ql[i], a, 0, 0, 0);
+            for (int w = 0; w < 4; w++) {
+                h[w] = pack_f16(__builtin_ldexpf(x[i][w], up - 4 * (w & 1)), __builtin_ldexpf(x[i][w + 4], up - 4 * (w & 1)));
             }
-#pragma unroll
-            for (int e = 0; e < 4; e++) sc[4 * b + e] = __builtin_fmaf(a[e], scale_of(kp[4 * b + e]), qsum * zero_of(kp[4 * b + e]));
+            if constexpr (KEPT) q[b][i] = __builtin_bit_cast(v8h, h);
+            else mine_q[(b * ND + i) * 64] = h;
         }
-        if (t0 + 32 > least || !__all(there)) {
+        qsum[b] = __builtin_ldexpf(sum, up - 24);   // scores are in units of 2^(24 - up)
+        unit[b] = fminf(fmaxf(__builtin_ldexpf(p.scale2, 24 - up), 0x1p-126f), 0x1.fffffep127f);
+    }
+    v4f o[CB][NB], wsum[CB];
+    float m[CB], limit[CB], l[CB], zsum[CB];   // m: what the weights are relative to, a power of two
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (!there || t0 + 8 * g + e >= seen) sc[e] = -__builtin_inff(), vp[e] = 0u;   // what lies there is not looked at
+    for (int b = 0; b < CB; b++) {
+#pragma unroll
+        for (int i = 0; i < NB; i++) o[b][i] = v4f{0, 0, 0, 0};
+        wsum[b] = v4f{0, 0, 0, 0}, m[b] = limit[b] = -__builtin_inff(), l[b] = zsum[b] = 0.0f;
+    }
+    const v4u eights = {0x00080008u, 0x00800080u, 0x00080008u, 0x00800080u};   // 8 in units of the codes
+    int vexp = 6;   // biased exponent of the largest vs so far: weights are scaled by 2^(131 - vexp)
+
+    // EDGE: some row does not see all of the step's tokens
+    // keys_done, values_done: called when those of the step are not needed any more
+    auto compute = [&](Kv4Step<D>& x, int t0, auto edge, auto keys_done, auto values_done) {
+        constexpr bool EDGE = decltype(edge)::value;
+        float vs[8], vz[8];
+        if (EDGE) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x.vp[e] = x.there && t0 + 8 * g + e < held ? x.vp[e] : 0u;   // behind the sequence: not looked at
         }
-        float top = m;
+        float largest = 0.0f;   // (NaN, the scale of a token of NaN, is passed over)
 #pragma unroll
-        for (int e = 0; e < 8; e++) top = fmaxf(top, sc[e]);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float safe = top == -__builtin_inff() ? 0.0f : top;
-        if (__any(top > m)) {
-            const float f = __builtin_amdgcn_exp2f((m - safe) * p.scale2);
-            l *= f, zsum *= f, wsum *= f;
-#pragma unroll
-            for (int i = 0; i < NB; i++) o[i] *= f;
-            m = top;
-        }
-        float w[8];
+        for (int e = 0; e < 8; e++) largest = fmaxf(largest, scale_of(x.vp[e]));
+        largest = max_over_quarters(largest);
+        const int grown = __builtin_amdgcn_readfirstlane(max(vexp, min((int)(__builtin_bit_cast(uint32_t, largest) >> 23), 254)));   // (columns share their tokens)
+        const float shrink = grown != vexp ? power(max(127 - (grown - vexp), 0)) : 1.0f;
+        const bool new_scale = grown != vexp;
+        vexp = grown;
+        const float even = power(258 - vexp), odd = even * 0.0625f;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const float x = __builtin_amdgcn_exp2f((sc[e] - safe) * p.scale2);
-            l += x;
-            zsum = __builtin_fmaf(x, __builtin_fmaf(8.0f, scale_of(vp[e]), zero_of(vp[e])), zsum);
-            w[e] = x * scale_of(vp[e]);
+            const float sc = scale_of(x.vp[e]);
+            vz[e] = __builtin_fmaf(8.0f, sc, zero_of(x.vp[e]));
+            vs[e] = sc * ((e & 1) ? odd : even);
         }
-        v8bf wh, wl;
-        split8<PARTS>(w, wh, wl);
-        wsum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, wh, wsum, 0, 0, 0);
-        if (PARTS == 2) wsum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, wl, wsum, 0, 0, 0);
+        float sc[CB][8];
+        {
+            v4f a[2][CB];
 #pragma unroll
-        for (int i = 0; i < NB; i++) {
-            const v8bf a = codes8(vw[i]);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, wh, o[i], 0, 0, 0);
-            if (PARTS == 2) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, wl, o[i], 0, 0, 0);
+            for (int i = 0; i < ND; i++) {
+                const v8h k0 = codes8(x.kw[0][i]), k1 = codes8(x.kw[1][i]);
+#pragma unroll
+                for (int cb = 0; cb < CB; cb++) {
+                    v8h qi;
+                    if constexpr (KEPT) qi = q[cb][i];
+                    else qi = __builtin_bit_cast(v8h, mine_q[(cb * ND + i) * 64]);
+                    if (i == 0) a[0][cb] = a[1][cb] = v4f{0, 0, 0, 0};
+                    a[0][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qi, a[0][cb], 0, 0, 0);
+                    a[1][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qi, a[1][cb], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float ks = scale_of(x.kp[4 * b + e]), kz = zero_of(x.kp[4 * b + e]);
+#pragma unroll
+                    for (int cb = 0; cb < CB; cb++) sc[cb][4 * b + e] = __builtin_fmaf(a[b][cb][e], ks, qsum[cb] * kz);
+                }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        keys_done();
+        v8h wh[CB], wl[PARTS == 2 ? CB : 1];
+#pragma unroll
+        for (int cb = 0; cb < CB; cb++) {
+            if (EDGE) {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (!x.there || t0 + 8 * g + e >= seen[cb]) sc[cb][e] = -__builtin_inff();
+            }
+            float top = sc[cb][0];
+#pragma unroll
+            for (int e = 1; e < 8; e++) top = fmaxf(top, sc[cb][e]);
+            top = max_over_quarters(top);
+            // what the weights are relative to moves when it is passed by more than 2^8 (and by the first tokens that a row sees): they and their sums
+            // have room for that, and most steps need not touch the sums (500 -> 364 us, with the steps that look at each token in a loop of their own)
+            if (new_scale || __any(top * unit[cb] > limit[cb])) {
+                const bool move = top * unit[cb] > limit[cb];
+                const float to = move ? top * unit[cb] : m[cb], f = move ? __builtin_amdgcn_exp2f(m[cb] - to) : 1.0f, fo = f * shrink;
+                l[cb] *= f, zsum[cb] *= f, wsum[cb] *= fo;
+#pragma unroll
+                for (int i = 0; i < NB; i++) o[cb][i] *= fo;
+                m[cb] = to, limit[cb] = to + 8.0f;
+            }
+            const float off = m[cb] == -__builtin_inff() ? 0.0f : -m[cb];
+            uint32_t hi[4], lo[4];
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[cb][e], unit[cb], off));
+                l[cb] += y;
+                const bool hidden = EDGE && (!x.there || t0 + 8 * g + e >= seen[cb]);   // what a row does not see may be no number
+                zsum[cb] = hidden ? zsum[cb] : __builtin_fmaf(y, vz[e], zsum[cb]);
+                w[e] = hidden ? 0.0f : y * vs[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                hi[e] = pack_f16(w[e], w[e + 4]);
+                if (PARTS == 2) {
+                    const v2f h = unpack_f16(hi[e]);
+                    lo[e] = pack_f16(w[e] - h[0], w[e + 4] - h[1]);
+                }
+            }
+            wh[cb] = __builtin_bit_cast(v8h, (v4u{hi[0], hi[1], hi[2], hi[3]}));
+            if (PARTS == 2) wl[PARTS == 2 ? cb : 0] = __builtin_bit_cast(v8h, (v4u{lo[0], lo[1], lo[2], lo[3]}));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i <= NB; i++) {
+            const v8h a = i == NB ? __builtin_bit_cast(v8h, eights) : codes8(x.vw[i == NB ? 0 : i]);
+#pragma unroll
+            for (int cb = 0; cb < CB; cb++) {
+                v4f& to = i == NB ? wsum[cb] : o[cb][i == NB ? 0 : i];
+                to = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wh[cb], to, 0, 0, 0);
+                if (PARTS == 2) to = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wl[PARTS == 2 ? cb : 0], to, 0, 0, 0);
+            }
+        }
+        values_done();
+    };
+    // Steps below `plain` are seen by all rows, in pages of the cache.  What is left, the last step or two, looks at each token; so does everything where
+    // the table has a bad page.
+    const int plain = from < to && seq.all_there((from * 32) >> kv.shift, (to * 32 - 1) >> kv.shift) ? min(to, least / 32) : 0;
+    auto nothing = []() {};
+    if constexpr (WT == 1) {
+        Kv4Place at;
+        auto keys = [&]() {
+            if (st + 1 < to) at = place_of(seq, (st + 1) * 32), ring[0].fetch_keys(seq, at, (st + 1) * 32, c, g);
+        };
+        auto values = [&]() {
+            if (st + 1 < to) ring[0].fetch_values(seq, at, (st + 1) * 32, c, g);
+        };
+        for (; st < plain; st++) compute(ring[0], st * 32, std::false_type{}, keys, values);
+        for (; st < to; st++) compute(ring[0], st * 32, std::true_type{}, keys, values);
+    } else {
+        for (; st + (AHEAD - 1) * WT < plain; st += AHEAD * WT)
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                compute(ring[i], (st + i * WT) * 32, std::false_type{}, nothing, nothing);
+                if (st + (i + AHEAD) * WT < to) fetch(ring[i], st + (i + AHEAD) * WT);
+            }
+        for (; st < to; st += AHEAD * WT)
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                if (st + i * WT < to) compute(ring[i], (st + i * WT) * 32, std::true_type{}, nothing, nothing);
+                if (st + (i + AHEAD) * WT < to) fetch(ring[i], st + (i + AHEAD) * WT);
+            }
+    }
+    // channel (4 g + e) NB + i of a row is in accumulator e of block i
+    const float back = power(vexp - 4);   // 1 / the weights' scale, and 2^24 for the codes
+    auto row_at = [&](uint32_t r) { return (int64_t)(first + (int)(r / group)) * p.heads_q + head * p.group + (int)(r % group); };
+#pragma unroll
+    for (int b = 0; b < CB; b++) {
+        l[b] = sum_over_quarters(l[b]), zsum[b] = sum_over_quarters(zsum[b]);
+        if constexpr (WT == 1) {
+            const uint32_t r = row0 + 16 * b + c;
+            if (r >= rows) continue;
+            const int64_t at = row_at(r);
+            const float f = l[b] == 0.0f ? 0.0f : 1.0f / l[b];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                T v[NB];
+#pragma unroll
+                for (int i = 0; i < NB; i++) v[i] = (T)(l[b] == 0.0f ? 0.0f : __builtin_fmaf((o[b][i][e] - wsum[b][e]) * 0x1p24f, back, zsum[b]) * f);
+                __builtin_memcpy(static_cast<T*>(p.out) + at * D + (4 * g + e) * NB, v, sizeof(v));
+            }
+        } else {   // the wavefronts meet
+            constexpr int LD = D + 4;
+            float* const mine = lds + (wave * TILE + 16 * b + c) * LD;
+#pragma unroll
+            for (int i = 0; i < NB; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) mine[(4 * g + e) * NB + i] = __builtin_fmaf((o[b][i][e] - wsum[b][e]) * 0x1p24f, back, zsum[b]);
+            float* const ml = lds + WT * TILE * LD;
+            if (g == 0) ml[(wave * TILE + 16 * b + c) * 2] = m[b], ml[(wave * TILE + 16 * b + c) * 2 + 1] = l[b];
         }
     }
-    l += __shfl_xor(l, 16), zsum += __shfl_xor(zsum, 16);
-    l += __shfl_xor(l, 32), zsum += __shfl_xor(zsum, 32);
-    // the wavefronts meet: sums of a row, channel (4 g + e) NB + i of block i in accumulator e
-    constexpr int LD = D + 4;
-    float* const mine = lds + (wave * 16 + c) * LD;
+    if constexpr (WT > 1) {
+        constexpr int LD = D + 4;
+        const int64_t all = (int64_t)kv.tokens * p.heads_q;
+        const float* const ml = lds + WT * TILE * LD;
+        __syncthreads();
+        for (int x = threadIdx.x; x < TILE * D; x += 64 * WT) {
+            const int r = x / D, d = x % D;
+            const uint32_t rr = row0 + r;
+            if (rr >= rows) break;
+            float top = -__builtin_inff(), sum = 0.0f, den = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NB; i++)
+            for (int w = 0; w < WT; w++) top = fmaxf(top, ml[(w * TILE + r) * 2]);
+            const float safe = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
-        for (int e = 0; e < 4; e++) mine[(4 * g + e) * NB + i] = o[i][e] - 136.0f * wsum[e] + zsum;
-    float* const ml = lds + WAVES * 16 * LD;
-    if (g == 0) ml[(wave * 16 + c) * 2] = m, ml[(wave * 16 + c) * 2 + 1] = l;
-    __syncthreads();
-    for (int x = threadIdx.x; x < 16 * D; x += 256) {
-        const int r = x / D, d = x % D;
-        const int64_t rr = (int64_t)tile * kTile + r;
-        if (rr >= rows) break;
-        float top = -__builtin_inff(), sum = 0.0f, den = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) top = fmaxf(top, ml[(w * 16 + r) * 2]);
-        const float safe = top == -__builtin_inff() ? 0.0f : top;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            const float f = __builtin_amdgcn_exp2f((ml[(w * 16 + r) * 2] - safe) * p.scale2);
-            sum = __builtin_fmaf(lds[(w * 16 + r) * LD + d], f, sum);
-            den = __builtin_fmaf(ml[(w * 16 + r) * 2 + 1], f, den);
-        }
-        const int64_t at = (int64_t)(first + rr / p.group) * p.heads_q + head * p.group + rr % p.group;
-        if (p.splits == 1) {
-            static_cast<T*>(p.out)[at * D + d] = (T)(den == 0.0f ? 0.0f : sum / den);
-        } else {
-            const int64_t all = (int64_t)kv.tokens * p.heads_q;
-            p.part[(split * all + at) * D + d] = sum;
-            if (d == 0) {
-                float* const pm = p.part + p.splits * all * D + (split * all + at) * 2;
-                pm[0] = top, pm[1] = den;
+            for (int w = 0; w < WT; w++) {
+                const float lw = ml[(w * TILE + r) * 2 + 1];
+                const float f = lw == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[(w * TILE + r) * 2] - safe);
+                sum = __builtin_fmaf(lds[(w * TILE + r) * LD + d], f, sum);
+                den = __builtin_fmaf(lw, f, den);
+            }
+            const int64_t at = row_at(rr);
+            if (p.splits == 1) {
+                static_cast<T*>(p.out)[at * D + d] = (T)(den == 0.0f ? 0.0f : sum / den);
+            } else {
+                p.part[(split * all + at) * D + d] = sum;
+                if (d == 0) {
+                    float* const pm = p.part + p.splits * all * D + (split * all + at) * 2;
+                    pm[0] = top, pm[1] = den;
+                }
             }
         }
     }
 }
 
-// the parts of a row meet
+// The parts of a row meet: a workgroup per row, D / 4 lanes on its channels, so that 256 / (D / 4) parts are read at a time.
 template <typename T, int D>
-__global__ __launch_bounds__(64) void k_kv4_join(Kv4Attend p) {
+__global__ __launch_bounds__(256) void k_kv4_join(Kv4Attend p) {
+    constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+    __shared__ v4f sums[GROUPS][LANES];
+    __shared__ float weight[64], total;
     const int64_t all = (int64_t)p.kv.tokens * p.heads_q, at = blockIdx.x;
-    const int token = (int)(at / p.heads_q);
-    if (token < p.kv.starts[0] || token >= p.kv.starts[p.kv.sequences]) return;
+    const int token = (int)((uint32_t)at / (uint32_t)p.heads_q);   // (below 2^31 rows)
+    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    static_assert(kMostSplits <= 64, "a lane per part");
+    // what all depends on is asked for at once: the first parts before their weights are known
     const float* const pm = p.part + p.splits * all * D;
-    float top = -__builtin_inff(), den = 0.0f, sum[(D + 63) / 64] = {};
-    for (int i = 0; i < p.splits; i++) top = fmaxf(top, pm[(i * all + at) * 2]);
-    const float safe = top == -__builtin_inff() ? 0.0f : top;
-    for (int i = 0; i < p.splits; i++) {
-        const float f = __builtin_amdgcn_exp2f((pm[(i * all + at) * 2] - safe) * p.scale2);
-        den = __builtin_fmaf(pm[(i * all + at) * 2 + 1], f, den);
+    const bool mine = (int)threadIdx.x < p.splits;   // (the first wavefront's lanes)
+    const float m = mine ? pm[(threadIdx.x * all + at) * 2] : -__builtin_inff(), l = mine ? pm[(threadIdx.x * all + at) * 2 + 1] : 0.0f;
+    constexpr int EARLY = 4;
+    v4f x[EARLY];
 #pragma unroll
-        for (int x = 0; x < (D + 63) / 64; x++)
-            if (x * 64 + lane_id() < D) sum[x] = __builtin_fmaf(p.part[(i * all + at) * D + x * 64 + lane_id()], f, sum[x]);
+    for (int i = 0; i < EARLY; i++) x[i] = *reinterpret_cast<const v4f*>(p.part + (min(group + i * GROUPS, p.splits - 1) * all + at) * D + 4 * lane);
+    if (token < p.kv.starts[0] || token >= p.kv.starts[p.kv.sequences]) return;   // (the whole workgroup)
+    if (threadIdx.x < 64) {
+        float top = m;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        const float w = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        float den = w * l;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) den += __shfl_xor(den, d);
+        weight[threadIdx.x] = w;
+        if (threadIdx.x == 0) total = den;
     }
+    __syncthreads();
+    v4f sum = {0, 0, 0, 0};
+    if (group < GROUPS) {
 #pragma unroll
-    for (int x = 0; x < (D + 63) / 64; x++)
-        if (x * 64 + lane_id() < D) static_cast<T*>(p.out)[at * D + x * 64 + lane_id()] = (T)(den == 0.0f ? 0.0f : sum[x] / den);
+        for (int i = 0; i < EARLY; i++) {
+            const float w = group + i * GROUPS < p.splits ? weight[group + i * GROUPS] : 0.0f;
+            sum += w == 0.0f ? v4f{0, 0, 0, 0} : w * x[i];
+        }
+        for (int i = group + EARLY * GROUPS; i < p.splits; i += GROUPS) {
+            const v4f y = *reinterpret_cast<const v4f*>(p.part + (i * all + at) * D + 4 * lane);
+            const float w = weight[i];
+            sum += w == 0.0f ? v4f{0, 0, 0, 0} : w * y;
+        }
+        sums[group][lane] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x >= LANES) return;
+#pragma unroll
+    for (int i = 1; i < GROUPS; i++) sum += sums[i][lane];
+    T y[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = (T)(total == 0.0f ? 0.0f : sum[e] / total);
+    __builtin_memcpy(static_cast<T*>(p.out) + at * D + 4 * lane, y, sizeof(y));
 }
 
 // fn(the head size as a constant)
@@ -507,15 +748,28 @@ hipError_t with_dim(int dim, F&& fn) {
     }
 }
 
-int64_t tiles_of(const ftnn_kv4_t& kv, int group) {   // at most: tokens of a sequence share tiles, sequences do not
+// How a call is split.  Tiles of 16 rows, whose tokens the four wavefronts of a workgroup share, or, where that fills the chip, wavefronts of 32 rows (16
+// of dim 256) on all tokens: they read and unpack the cache once for twice the rows and have no partial sums to join.  Fewer workgroups than
+// run at once (two per compute unit, one of dim 256) split their tokens further, down to 512 each, and a second launch joins the parts.  us, 16 / 32 rows,
+// 8 heads of 4 x 128 at a length of 4000: 512 new tokens 83 / 102, 1024 156 / 187, 2048 247 / 217; 4 x 512 at 2000 126 / 109.
+struct Kv4Plan {
+    int blocks, waves;   // CB, WT
+    int64_t tiles;
+    int splits;
+};
+int64_t tiles_of(const ftnn_kv4_t& kv, int group, int rows) {   // at most: tokens of a sequence share tiles, sequences do not
     const int64_t t = kv.tokens;
-    return std::min((t * group + kTile - 1) / kTile + kv.sequences, t * ((group + kTile - 1) / kTile));
+    return std::min((t * group + rows - 1) / rows + kv.sequences, t * ((group + rows - 1) / rows));
 }
-
-int splits_of(const ftnn_kv4_t& kv, int heads_q, int max_len) {
-    const int64_t most = max_len > 0 ? std::min<int64_t>(max_len, (int64_t)kv.width * kv.page) : (int64_t)kv.width * kv.page;
-    const int64_t base = std::max<int64_t>(1, tiles_of(kv, heads_q / kv.heads) * kv.heads);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({512 / base, (most + 255) / 256, 64}));
+Kv4Plan plan_of(const ftnn_kv4_t& kv, int heads_q, int max_len) {
+    const int group = heads_q / kv.heads;
+    const int64_t capacity = (int64_t)kv.width * kv.page, most = max_len > 0 ? std::min<int64_t>(max_len, capacity) : capacity;
+    const int64_t resident = kv.dim == 256 ? 240 : 512, least = 512;
+    auto splits = [&](int64_t tiles) { return (int)std::max<int64_t>(1, std::min<int64_t>({resident / std::max<int64_t>(1, tiles * kv.heads), (most + least - 1) / least, kMostSplits})); };
+    const int blocks = kv.dim <= 128 ? 2 : 1;
+    const int64_t wide = tiles_of(kv, group, 64 * blocks), narrow = tiles_of(kv, group, 16);
+    if ((int64_t)kv.tokens * group / (64 * blocks) * kv.heads >= 480) return {blocks, 1, wide, 1};
+    return {1, 4, narrow, splits(narrow)};
 }
 
 }  // namespace
@@ -544,27 +798,36 @@ hipError_t launch_kv4_read(const ftnn_kv4_t& kv, int dtype, void* d_k, void* d_v
 }
 
 int64_t kv4_attention_scratch(const ftnn_kv4_t& kv, int heads_q, int max_len) {
-    const int64_t splits = splits_of(kv, heads_q, max_len);
+    const int64_t splits = plan_of(kv, heads_q, max_len).splits;
     return splits == 1 ? 0 : splits * kv.tokens * heads_q * (kv.dim + 2) * 4;
 }
 
 hipError_t launch_kv4_attention(const ftnn_kv4_t& kv, int dtype, int heads_q, const Kv4Rows& q, float scale, int max_len, void* d_out,
                                 void* d_scratch, hipStream_t st) {
+    const Kv4Plan plan = plan_of(kv, heads_q, max_len);
     Kv4Attend p;
-    p.kv = device_view(kv), p.q = q, p.heads_q = heads_q, p.group = heads_q / kv.heads, p.splits = splits_of(kv, heads_q, max_len);
+    p.kv = device_view(kv), p.q = q, p.heads_q = heads_q, p.group = heads_q / kv.heads, p.splits = plan.splits;
     p.scale2 = scale * 1.44269504088896341f, p.out = d_out, p.part = static_cast<float*>(d_scratch);
-    const int64_t tiles = tiles_of(kv, p.group);
     auto go = [&](auto t) {
         typedef decltype(t) T;
         return with_dim(kv.dim, [&](auto d) {
             constexpr int D = decltype(d)::value;
-            const size_t bytes = 4 * 16 * (D + 4 + 2) * 4;
-            static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(k_kv4_attend<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 << 10);
-            if (set != hipSuccess) return set;
-            k_kv4_attend<T, D><<<dim3((unsigned)tiles, kv.heads, p.splits), dim3(256), bytes, st>>>(p);
-            hipError_t e = hipGetLastError();
+            auto run = [&](auto cb, auto wt) {
+                constexpr int CB = decltype(cb)::value, WT = decltype(wt)::value, bytes = WT == 1 ? 4 * CB * (D / 32) * 1024 : WT * 16 * CB * (D + 4 + 2) * 4;
+                auto* const kern = k_kv4_attend<T, D, CB, WT>;
+                static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, std::max(bytes, 16));
+                if (set != hipSuccess) return set;
+                kern<<<dim3((unsigned)plan.tiles, kv.heads, plan.splits), dim3(WT == 1 ? 256 : 64 * WT), bytes, st>>>(p);
+                return hipGetLastError();
+            };
+            using One = std::integral_constant<int, 1>;
+            using Two = std::integral_constant<int, 2>;
+            hipError_t e;
+            if (plan.waves == 4) e = run(One{}, std::integral_constant<int, 4>{});
+            else if constexpr (D <= 128) e = run(Two{}, One{});
+            else e = run(One{}, One{});
             if (e != hipSuccess || p.splits == 1) return e;
-            k_kv4_join<T, D><<<dim3((unsigned)((int64_t)kv.tokens * heads_q)), dim3(64), 0, st>>>(p);
+            k_kv4_join<T, D><<<dim3((unsigned)((int64_t)kv.tokens * heads_q)), dim3(256), 0, st>>>(p);
             return hipGetLastError();
         });
     };

@@ -422,7 +422,7 @@ typedef struct ftnn_kv4 {
     int64_t pages;          /* pages in the cache                           */
     int heads, dim, page;   /* heads of keys and values; tokens per page    */
     int sequences, tokens;  /* sequences; rows of the call's tensors        */
-    int width;              /* pages that a sequence may have               */
+    int width;              /* pages that a sequence may have, 2^30 tokens at most */
     int64_t table_stride;   /* entries between sequences of the table       */
     const int32_t *d_table; /* [sequences][width]                           */
     const int32_t *d_lens;  /* [sequences]                                  */
@@ -455,8 +455,8 @@ FTNN_API int ftnn_kv4_read(const ftnn_kv4_t *kv, int dtype, void *d_k, void *d_v
  * head j / (heads_q / heads)): softmax(scale q k) v over the tokens up to the query's own.  d_out: [tokens][heads_q][dim],
  * contiguous, of the queries' type (FTNN_F16 or FTNN_BF16); zeros for a query that sees no token.  max_len: the largest of lens if the
  * caller knows it, else 0; it decides how the work is split and nothing else.  d_scratch: 16-byte aligned,
- * ftnn_kv4_attention_scratch_bytes() bytes (0: none needed).  Products are computed in bfloat16 with fp32 sums, queries and
- * weights of FTNN_F16 as two bfloat16 each.
+ * ftnn_kv4_attention_scratch_bytes() bytes (0: none needed).  Products are computed in float16 with fp32 sums, the
+ * weights of FTNN_F16 as two float16 each.
  */
 FTNN_API int64_t ftnn_kv4_attention_scratch_bytes(const ftnn_kv4_t *kv, int heads_q, int max_len);
 FTNN_API int ftnn_kv4_attention(const ftnn_kv4_t *kv, int dtype, int heads_q, const void *d_q, int64_t q_token_stride,

@@ -187,6 +187,24 @@ def test_attention(heads, group, dim, page, lens, new, dtype):
     _attend(dim + page + len(lens), heads, group, dim, page, lens, new, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,group,dim,page,lens,new", [(32, 2, 64, 16, [700, 300, 200], [600, 300, 123]), (16, 4, 128, 64, [990, 64, 1], [900, 64, 1]),
+                                                           (16, 5, 96, 32, [500, 420], [400, 419]), (8, 4, 256, 16, [1000, 70], [930, 70])])
+def test_attention_of_many_rows(heads, group, dim, page, lens, new, dtype):
+    """enough rows to fill the chip with wavefronts on all tokens each"""
+    assert sum(new) * group // (64 if dim == 256 else 128) * heads >= 480
+    _attend(dim, heads, group, dim, page, lens, new, dtype, tokens=sum(new) + 3)
+
+
+def test_attention_of_many_rows_with_holes():
+    """bad pages in the middle, at the end and for all of a sequence; garbage behind the sequences"""
+    def change(raw, table, ln, st):
+        raw[table[0, 9].item()] = 255   # NaN
+        ln[0] = 575                     # in the page behind
+        table[0, 3], table[0, 8], table[1, 0], table[2] = -1, raw.shape[0], 1 << 30, -5
+    _attend(25, 16, 4, 128, 64, [640, 300, 200], [500, 300, 200], "bf16", change=change)
+
+
 @pytest.mark.parametrize("max_len", [0, 1, 3000, 100000])
 def test_attention_over_a_long_cache(max_len):
     """split over workgroups, whatever the hint says"""

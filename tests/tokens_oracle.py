@@ -129,6 +129,7 @@ def attention(cache, table, lens, starts, q, scale=None):
                scale the relative error of a weight, and 2^-21 for the power of two
       weights  rounded to a unit of 2^-8 (float16: 2^-16 by two parts) where they meet code - 8
       sums     fp32 over steps of 32 tokens, of terms up to 143 + 136 times scale * weight
+    (a bound for products in bfloat16 with an offset of 128; ones in float16 without it are well inside)
       result   half a step of its type (below its normal numbers: of the smallest of those)"""
     tokens, heads_q, dim = q.shape
     group, scale = heads_q // cache.heads, dim ** -0.5 if scale is None else scale
@@ -154,13 +155,14 @@ def attention(cache, table, lens, starts, q, scale=None):
             blind = hidden.all(1)
             p = torch.softmax(score.masked_fill(blind[:, None], 0.0), 1).masked_fill(blind[:, None], 0.0)
             p = p.masked_fill(hidden, 0.0)
-            seen = ~hidden
-            clean = lambda a, m: torch.where(m, a, 0.0)   # what a row does not see adds nothing, whatever it is
-            o = torch.stack([p[r][seen[r]] @ v[seen[r]] for r in range(len(p))])
-            rel = scale * (dim + 8) * u * x.abs().sum(1) * torch.stack([clean((143 * kp[:, 0] + kp[:, 1].abs()), m).nan_to_num().amax() for m in seen]) + 2.0 ** -21
-            vmax = torch.stack([clean(v.abs().amax(1), m).nan_to_num().amax() for m in seen])
-            round_w = torch.stack([p[r][seen[r]] @ (vp[seen[r], :1] * (cache.v[page, h, i][seen[r]].double() - 8).abs()) for r in range(len(p))])
-            sums = torch.stack([p[r][seen[r]] @ vp[seen[r], 0] for r in range(len(p))])[:, None] * 279 * (len(at) / 32 + 64) * u
+            looked = (~hidden).any(0)   # what no row sees adds nothing, whatever it is
+            kp, vp, v = (torch.where(looked[:, None], a, 0.0) for a in (kp, vp, v))
+            o = p @ v
+            most = lambda a: torch.where(hidden, 0.0, a).amax(1)   # of what a row sees
+            rel = scale * (dim + 8) * u * x.abs().sum(1) * most(143 * kp[:, 0] + kp[:, 1].abs()) + 2.0 ** -21
+            vmax = most(v.abs().amax(1))
+            round_w = p @ (vp[:, :1] * (cache.v[page, h, i].double() - 8).abs())
+            sums = (p @ vp[:, 0])[:, None] * 279 * (len(at) / 32 + 64) * u
             e = unit * round_w + 4 * rel[:, None] * vmax[:, None] + sums + o.abs() * (torch.finfo(q.dtype).eps / 2 + 8 * u) + torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps / 2
             out[first:last, h * group:(h + 1) * group] = o.view(last - first, group, dim)
             slack[first:last, h * group:(h + 1) * group] = e.view(last - first, group, dim)
