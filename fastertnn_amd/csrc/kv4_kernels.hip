@@ -46,29 +46,38 @@ Kv4 device_view(const ftnn_kv4_t& k) {
 
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 63; }
 
-// the sequence of token row t, or -1 behind the last one: a wavefront compares 64 starts at a time
-__device__ __forceinline__ int sequence_of(const Kv4& kv, int t) {
-    int lo = 0, n = kv.sequences;
-    while (n > 0) {
-        const int stride = (n + 63) / 64, i = min((lane_id() + 1) * stride, n);
-        const int c = __popcll(__ballot(lane_id() * stride < n && kv.starts[lo + i] <= t));
-        lo += min(c * stride, n);
-        n = min(stride, n - min(c * stride, n));
-        if (stride == 1) break;
+// The tokens of a call that share a block of 8 positions: their rows t .. t + count - 1 of sequence s, from position pos on.  The values of a block lie in
+// the same words, so it has one owner: number `number` of the call's blocks, counted sequence by sequence.  count is 0 behind the last.
+struct Kv4Eight {
+    int s, t, count, pos;
+};
+__device__ __forceinline__ Kv4Eight find_eight(const Kv4& kv, int number) {
+    int before = 0;
+    for (int b0 = 0; b0 < kv.sequences; b0 += 64) {
+        const int b = min(b0 + lane_id(), kv.sequences - 1);
+        const int from = kv.starts[b], to = kv.starts[b + 1], length = kv.lens[b], first = max(from, 0), end = min(to, kv.tokens);   // together: one wait
+        // position of row `first`; negative where a sequence has more new tokens than it holds: its blocks are counted too
+        const int pos = max(length, 0) - to + first, rows = b0 + lane_id() < kv.sequences ? end - first : 0;
+        const int blocks = rows > 0 ? ((pos + rows - 1) >> 3) - (pos >> 3) + 1 : 0;
+        int sum = blocks;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int o = __shfl_up(sum, d);
+            if (lane_id() >= d) sum += o;
+        }
+        const uint64_t past = __ballot(before + sum > number);
+        if (past) {
+            const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)past) - 1);
+            auto at = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            const int row0 = at(first), n = at(rows), p0 = at(pos), i = number - before - at(sum) + at(blocks), done = i == 0 ? 0 : 8 * i - (p0 & 7);
+            return {b0 + l, row0 + done, min(8 - ((p0 + done) & 7), n - done), p0 + done};
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
     }
-    return lo < kv.sequences ? lo : -1;
+    return {0, 0, 0, 0};
 }
-
-// The tokens of a call that share a block of 8 positions, which the first of them stands for: count of them from row t on, or 0
-// where t is not the first.  pos: of row t.
-__device__ __forceinline__ int tokens_of_eight(const Kv4& kv, int t, int* s, int64_t* pos) {
-    *s = sequence_of(kv, t);
-    if (*s < 0) return 0;
-    const int first = kv.starts[*s], end = min(kv.starts[*s + 1], kv.tokens);
-    *pos = (int64_t)kv.lens[*s] - kv.starts[*s + 1] + t;
-    if (t != first && (*pos & 7) != 0) return 0;
-    return min(8 - (int)(*pos & 7), end - t);
-}
+// blocks of 8 positions at most: a sequence's first and last may be cut
+int eights_of(const ftnn_kv4_t& kv) { return (int)std::min<int64_t>(kv.tokens, ((int64_t)kv.tokens + 7) / 8 + 2 * (int64_t)kv.sequences); }
 
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
@@ -87,23 +96,44 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 
 // values d .. d + 7 of a row at position pos, rotated: products and sums in 64 bits, one rounding to fp32
 template <typename T>
-__device__ __forceinline__ void load_rotated(const T* row, int d, int64_t pos, const Kv4Rotation& r, float (&y)[8]) {
-    float x[8];
-    load8(row + d, x);
+__device__ __forceinline__ void load_rotated(const T* row, int d, int pos, const Kv4Rotation& r, float (&y)[8]) {
+    load8(row + d, y);
+    if (d >= r.rot) return;
     const int half = r.rot / 2;
-    const float *const c = r.cos + pos * half, *const n = r.sin + pos * half;
+    const float *const c = r.cos + (int64_t)pos * half, *const n = r.sin + (int64_t)pos * half;
+    float other[8], cv[8], nv[8];
+    bool second[8];
+    if (r.neighbours && d + 8 <= r.rot) {   // whole pairs, four entries of the tables
+        float c4[4], n4[4];
+        __builtin_memcpy(c4, c + d / 2, 16), __builtin_memcpy(n4, n + d / 2, 16);
+#pragma unroll
+        for (int i = 0; i < 8; i++) other[i] = y[i ^ 1], cv[i] = c4[i / 2], nv[i] = n4[i / 2], second[i] = i & 1;
+    } else if (!r.neighbours && half % 8 == 0) {   // the other halves lie together
+        const bool late = d >= half;
+        const int at = late ? d - half : d;
+        load8(row + (late ? at : d + half), other);
+        __builtin_memcpy(cv, c + at, 32), __builtin_memcpy(nv, n + at, 32);
+#pragma unroll
+        for (int i = 0; i < 8; i++) second[i] = late;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int e = min(d + i, r.rot - 1);   // (what is behind stays as it is)
+            second[i] = r.neighbours ? (e & 1) : e >= half;
+            const int at = r.neighbours ? e / 2 : second[i] ? e - half : e;
+            other[i] = r.neighbours ? y[i ^ 1] : (float)row[second[i] ? e - half : e + half];
+            cv[i] = c[at], nv[i] = n[at];
+        }
+    }
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const int e = d + i;
-        if (e >= r.rot) {
-            y[i] = x[i];
-            continue;
-        }
-        const bool second = r.neighbours ? (e & 1) : e >= half;
-        const int at = r.neighbours ? e / 2 : second ? e - half : e;
-        const double other = r.neighbours ? (double)x[i ^ 1] : (double)(float)row[second ? e - half : e + half];
-        const double a = (double)x[i] * (double)c[at], b = other * (double)n[at];   // exact
-        y[i] = (float)(second ? a + b : a - b);
+        if (d + i >= r.rot) continue;
+        const double a = (double)y[i] * (double)cv[i], b = (double)other[i] * (double)nv[i];   // exact
+        other[i] = (float)(second[i] ? a + b : a - b);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if (d + i < r.rot) y[i] = other[i];
         asm volatile("" : "+v"(y[i]));   // in fp32 from here on: the compiler would make one rounding of this and a caller's to 16 bits
     }
 }
@@ -121,11 +151,28 @@ __device__ __forceinline__ uint32_t make_params(float low, float high, bool fine
 __device__ __forceinline__ float scale_of(uint32_t params) { return __builtin_bit_cast(float, params << 16); }
 __device__ __forceinline__ float zero_of(uint32_t params) { return __builtin_bit_cast(float, params & 0xFFFF0000u); }
 
-// code of a value: in 64 bits, so that values next to a border come out as the formula says
-__device__ __forceinline__ uint32_t code_of(float x, float scale, float zero) {
+// Eight codes.  A difference, a reciprocal and a product in fp32 are off by less than 4 * 2^-24 of a quotient of up to 16, 2^-18: where none of the eight is
+// within 2^-16 of a border between codes they are what the formula says.  Others are divided in 64 bits.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float scale, float zero) {
     if (!(scale > 0.0f)) return 0;
-    const double q = __builtin_rint(((double)x - (double)zero) / (double)scale);
-    return (uint32_t)__builtin_fmin(__builtin_fmax(q, 0.0), 15.0);
+    const float inv = 1.0f / scale;
+    uint32_t w = 0;
+    bool near = !(inv < __builtin_inff());
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float q = (x[e] - zero) * inv, n = __builtin_rintf(q);
+        near |= !(q <= 17.0f) || __builtin_fabsf(__builtin_fabsf(q - n) - 0.5f) < 0x1p-16f;   // (more than 17: the difference is beyond fp32)
+        w |= (uint32_t)__builtin_fminf(__builtin_fmaxf(n, 0.0f), 15.0f) << (4 * e);
+    }
+    if (near) {
+        w = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const double q = __builtin_rint(((double)x[e] - (double)zero) / (double)scale);
+            w |= (uint32_t)__builtin_fmin(__builtin_fmax(q, 0.0), 15.0) << (4 * e);
+        }
+    }
+    return w;
 }
 
 template <int LG>
@@ -146,106 +193,119 @@ __device__ __forceinline__ void group_range(const float (&y)[8], bool live, floa
     *low = lo, *high = hi, *fine = ok;
 }
 
-// One wavefront per (block of 8 positions, head): blockIdx.x is a token row, which works if it is the first of its block;
-// blockIdx.y a head of keys and values, and behind those a head of queries.  The values of 8 tokens lie together, so the block has one
-// owner, and a call's other tokens in it come through LDS.
+// One wavefront per (block of 8 positions, head): four heads of keys and values, and behind those of queries, per workgroup.  LG lanes hold a token's
+// channels, eight each.  The codes of a block's values meet in LDS, where every lane makes the words of its channels; what the block holds already of
+// other tokens stays.
 template <typename T, int D>
-__global__ __launch_bounds__(64) void k_kv4_append(Kv4 kv, Kv4Rows k, Kv4Rows v, Kv4Rotation r, int heads_q, Kv4Rows q, T* q_out) {
+__global__ __launch_bounds__(256) void k_kv4_append(Kv4 kv, Kv4Rows k, Kv4Rows v, Kv4Rotation r, int heads_q, Kv4Rows q, T* q_out) {
     constexpr int LG = D <= 64 ? 8 : D <= 128 ? 16 : 32, TPI = 64 / LG;   // lanes of a token, tokens at a time
-    __shared__ __align__(8) uint8_t codes[8][D];
-    const int t = blockIdx.x, lane = lane_id(), li = lane % LG, d = 8 * li;
-    int s;
-    int64_t pos;
-    int count = tokens_of_eight(kv, t, &s, &pos);
-    if (count <= 0 || pos < 0) return;
-    if (r.rot && pos + count > r.positions) count = (int)max((int64_t)0, (int64_t)r.positions - pos);
-    if (count <= 0) return;
-    int head = blockIdx.y;
+    __shared__ uint32_t codes[4][8][D / 8];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane % LG, d = 8 * li;
+    int head = blockIdx.y * 4 + wave;
+    if (head >= kv.heads + heads_q) return;   // (nothing below waits for another wavefront)
+    const Kv4Eight at = find_eight(kv, blockIdx.x);
+    const int count = r.rot ? min(at.count, r.positions - at.pos) : at.count;
+    if (count <= 0 || at.pos < 0) return;
     if (head >= kv.heads) {
         head -= kv.heads;
-        for (int i = lane / LG; i < count; i += TPI)
-            if (d < D) {
+#pragma unroll
+        for (int i0 = 0; i0 < 8; i0 += TPI) {
+            const int i = i0 + lane / LG;
+            if (i < count && d < D) {
                 float y[8];
-                load_rotated(static_cast<const T*>(q.p) + (t + i) * q.token_stride + head * q.head_stride, d, pos + i, r, y);
-                store8(q_out + ((int64_t)(t + i) * heads_q + head) * D + d, y);
+                load_rotated(static_cast<const T*>(q.p) + (at.t + i) * q.token_stride + head * q.head_stride, d, at.pos + i, r, y);
+                store8(q_out + ((int64_t)(at.t + i) * heads_q + head) * D + d, y);
             }
+        }
         return;
     }
-    const int64_t id = kv.page_of(s, pos);
+    const int64_t id = kv.page_of(at.s, at.pos);
     if (id < 0) return;
     char* const block = kv.block(id, head);
-    const int slot = (int)(pos & (kv.page - 1));
-    for (int i0 = 0; i0 < count; i0 += TPI) {
-        const int i = i0 + lane / LG;
-        const bool live = i < count && d < D;
+    const int slot = at.pos & (kv.page - 1);
 #pragma unroll
-        for (int which = 0; which < 2; which++) {
-            float y[8] = {}, low, high, scale, zero;
+    for (int which = 0; which < 2; which++) {
+        float y[8 / TPI][8];   // all of the block is asked for at once
+#pragma unroll
+        for (int j = 0; j < 8 / TPI; j++) {
+            const int i = j * TPI + lane / LG;
+            if (i < count && d < D) {
+                if (which == 0) load_rotated(static_cast<const T*>(k.p) + (at.t + i) * k.token_stride + head * k.head_stride, d, at.pos + i, r, y[j]);
+                else load8(static_cast<const T*>(v.p) + (at.t + i) * v.token_stride + head * v.head_stride + d, y[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8 / TPI; j++) {
+            if (j * TPI >= count) break;
+            const int i = j * TPI + lane / LG;
+            const bool live = i < count && d < D;
+            float low, high, scale, zero;
             bool fine;
-            if (live) {
-                if (which == 0) load_rotated(static_cast<const T*>(k.p) + (t + i) * k.token_stride + head * k.head_stride, d, pos + i, r, y);
-                else load8(static_cast<const T*>(v.p) + (t + i) * v.token_stride + head * v.head_stride + d, y);
-            }
-            group_range<LG>(y, live, &low, &high, &fine);
+            group_range<LG>(y[j], live, &low, &high, &fine);
             const uint32_t params = make_params(low, high, fine, &scale, &zero);
-            if (!live) continue;
-            uint32_t w = 0;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint32_t c = code_of(y[e], scale, zero);
-                w |= c << (4 * e);
-                if (which == 1) codes[i][d + e] = (uint8_t)c;
+            if (live) {
+                const uint32_t w = codes_of(y[j], scale, zero);
+                if (which == 0) *reinterpret_cast<uint32_t*>(block + (slot + i) * (D / 2) + d / 2) = w;
+                else codes[wave][i][li] = w;
+                if (li == 0) *reinterpret_cast<uint32_t*>(block + (which ? kv.value_params() : kv.key_params()) + (slot + i) * 4) = params;
             }
-            if (which == 0) *reinterpret_cast<uint32_t*>(block + (slot + i) * (D / 2) + d / 2) = w;
-            if (li == 0) *reinterpret_cast<uint32_t*>(block + (which ? kv.value_params() : kv.key_params()) + (slot + i) * 4) = params;
         }
     }
-    __syncthreads();
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // the wavefront's own codes: its LDS accesses keep their order
+    __builtin_amdgcn_wave_barrier();
     uint32_t* const words = reinterpret_cast<uint32_t*>(block + kv.values()) + (slot / 8) * D;
-    const int at = slot & 7;
+    const int place = slot & 7;
     for (int e = lane; e < D; e += 64) {
         uint32_t w = 0;
-        for (int i = 0; i < count; i++) w |= (uint32_t)codes[i][e] << (4 * (at + i));
-        if (count < 8) w |= words[e] & ~((0xFFFFFFFFu >> (32 - 4 * count)) << (4 * at));
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < count) w |= (codes[wave][i][e / 8] >> (4 * (e & 7)) & 15u) << (4 * (place + i));
+        if (count < 8) w |= words[e] & ~((0xFFFFFFFFu >> (32 - 4 * count)) << (4 * place));
         words[e] = w;
     }
 }
 
+// the same blocks and lanes the other way round: a lane's eight channels of a token are one word of keys, and eight words that hold its token among others
 template <typename T, int D>
-__global__ __launch_bounds__(64) void k_kv4_read(Kv4 kv, T* K, T* V) {
+__global__ __launch_bounds__(256) void k_kv4_read(Kv4 kv, T* K, T* V) {
     constexpr int LG = D <= 64 ? 8 : D <= 128 ? 16 : 32, TPI = 64 / LG;
-    const int t = blockIdx.x, head = blockIdx.y, lane = lane_id(), d = 8 * (lane % LG);
-    int s;
-    int64_t pos;
-    const int count = tokens_of_eight(kv, t, &s, &pos);
-    if (count <= 0) return;
-    const int64_t id = pos >= 0 ? kv.page_of(s, pos) : -1;
+    const int lane = lane_id(), head = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = 8 * (lane % LG);
+    if (head >= kv.heads) return;
+    const Kv4Eight at = find_eight(kv, blockIdx.x);
+    if (at.count <= 0) return;
+    const int64_t id = at.pos >= 0 ? kv.page_of(at.s, at.pos) : -1;
     const char* const block = kv.block(max(id, (int64_t)0), head);
-    const int slot = (int)(pos & (kv.page - 1));
-    if (K)
-        for (int i = lane / LG; i < count; i += TPI)
-            if (d < D) {
-                float y[8] = {};
-                if (id >= 0) {
-                    const uint32_t w = *reinterpret_cast<const uint32_t*>(block + (slot + i) * (D / 2) + d / 2);
-                    const uint32_t p = *reinterpret_cast<const uint32_t*>(block + kv.key_params() + (slot + i) * 4);
+    const int slot = at.pos & (kv.page - 1);
+    const uint32_t* const words = reinterpret_cast<const uint32_t*>(block + kv.values()) + (slot / 8) * D + d;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) y[e] = __builtin_fmaf((float)(w >> (4 * e) & 15u), scale_of(p), zero_of(p));
-                }
-                store8(K + ((int64_t)(t + i) * kv.heads + head) * D + d, y);
+    for (int i0 = 0; i0 < 8; i0 += TPI) {
+        const int i = i0 + lane / LG;
+        if (i >= at.count || d >= D) continue;
+        const int64_t to = ((int64_t)(at.t + i) * kv.heads + head) * D + d;
+        if (K) {
+            float y[8] = {};
+            if (id >= 0) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(block + (slot + i) * (D / 2) + d / 2);
+                const uint32_t p = *reinterpret_cast<const uint32_t*>(block + kv.key_params() + (slot + i) * 4);
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = __builtin_fmaf((float)(w >> (4 * e) & 15u), scale_of(p), zero_of(p));
             }
-    if (V) {
-        const uint32_t* const words = reinterpret_cast<const uint32_t*>(block + kv.values()) + (slot / 8) * D;
-        for (int e = lane; e < D; e += 64) {
-            const uint32_t w = id >= 0 ? words[e] : 0u;
-            for (int i = 0; i < count; i++) {
-                const uint32_t p = id >= 0 ? *reinterpret_cast<const uint32_t*>(block + kv.value_params() + (slot + i) * 4) : 0u;
-                V[((int64_t)(t + i) * kv.heads + head) * D + e] = (T)__builtin_fmaf((float)(w >> (4 * ((slot + i) & 7)) & 15u), scale_of(p), zero_of(p));
+            store8(K + to, y);
+        }
+        if (V) {
+            float y[8] = {};
+            if (id >= 0) {
+                uint32_t w[8];
+                __builtin_memcpy(w, __builtin_assume_aligned(words, 16), 32);
+                const uint32_t p = *reinterpret_cast<const uint32_t*>(block + kv.value_params() + (slot + i) * 4);
+                const int shift = 4 * ((slot + i) & 7);
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = __builtin_fmaf((float)(w[e] >> shift & 15u), scale_of(p), zero_of(p));
             }
+            store8(V + to, y);
         }
     }
 }
-
 // ---------------------------------------------------------------------------------------------------------- attention
 //
 // Scores and outputs come from v_mfma_f32_16x16x32_f16 on the codes themselves.  A float16 whose bits are a code c is the subnormal number
@@ -780,7 +840,7 @@ hipError_t launch_kv4_append(const ftnn_kv4_t& kv, int dtype, const Kv4Rows& k, 
     return with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
         return with_dim(kv.dim, [&](auto d) {
-            k_kv4_append<T, decltype(d)::value><<<dim3(kv.tokens, kv.heads + heads_q), dim3(64), 0, st>>>(dv, k, v, r, heads_q, q, static_cast<T*>(d_q_out));
+            k_kv4_append<T, decltype(d)::value><<<dim3(eights_of(kv), (kv.heads + heads_q + 3) / 4), dim3(256), 0, st>>>(dv, k, v, r, heads_q, q, static_cast<T*>(d_q_out));
             return hipGetLastError();
         });
     });
@@ -791,7 +851,7 @@ hipError_t launch_kv4_read(const ftnn_kv4_t& kv, int dtype, void* d_k, void* d_v
     return with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
         return with_dim(kv.dim, [&](auto d) {
-            k_kv4_read<T, decltype(d)::value><<<dim3(kv.tokens, kv.heads), dim3(64), 0, st>>>(dv, static_cast<T*>(d_k), static_cast<T*>(d_v));
+            k_kv4_read<T, decltype(d)::value><<<dim3(eights_of(kv), (kv.heads + 3) / 4), dim3(256), 0, st>>>(dv, static_cast<T*>(d_k), static_cast<T*>(d_v));
             return hipGetLastError();
         });
     });
