@@ -185,7 +185,7 @@ __device__ __forceinline__ void unpack32(uint32_t s, uint32_t z, uint32_t (&out)
 
 // Few tokens: KS wavefronts split K over one tile of 16 NB weight rows x 16 MB tokens and meet in LDS.  Operands come straight from memory
 // into registers, the next step's while this one is multiplied.
-template <I8Weights W, typename T, int NB, int MB>
+template <I8Weights W, typename T, int NB, int MB, bool TOKENS>
 __global__ __launch_bounds__(512) void k_i8_few(I8Product p, uint32_t ntiles) {
     constexpr int KS = 8, LD = 16 * NB + 4;
     extern __shared__ __align__(16) int meet[];   // [KS][16 MB][LD]
@@ -248,39 +248,42 @@ __global__ __launch_bounds__(512) void k_i8_few(I8Product p, uint32_t ntiles) {
         const v4u* b[NB];
 #pragma unroll
         for (int j = 0; j < NB; j++) b[j] = static_cast<const v4u*>(p.b) + std::min<int64_t>(n0 + j * 16 + r, p.N - 1) * groups * (TERN ? 4 : 2);
-        v4u sn[NB], zn[NB];
-        auto fetch = [&](int q0) {
+        // what a step takes: the weights' planes, and of a few tokens (TOKENS) theirs, asked for a step ahead
+        static_assert(!TOKENS || MB == 1, "registers for one block of tokens");
+        struct Step {
+            v4u s[NB], z[NB];
+            v4i t[TOKENS ? 8 : 1];
+        };
+        auto fetch = [&](int q0, Step& x) {
             const int q = q0 + (g >> 1), half = g & 1;
             const bool in = q < groups;
 #pragma unroll
             for (int j = 0; j < NB; j++) {
-                sn[j] = in ? b[j][q * (TERN ? 4 : 2) + half] : v4u{0, 0, 0, 0};
-                zn[j] = TERN && in ? b[j][q * 4 + 2 + half] : v4u{0, 0, 0, 0};
+                x.s[j] = in ? b[j][q * (TERN ? 4 : 2) + half] : v4u{0, 0, 0, 0};
+                x.z[j] = TERN && in ? b[j][q * 4 + 2 + half] : v4u{0, 0, 0, 0};
+            }
+            if constexpr (TOKENS) {
+#pragma unroll
+                for (int d = 0; d < 8; d++) x.t[d] = token_piece(0, q * 256 + half * 128 + 16 * d);
             }
         };
-        int q0 = wave * 2;
-        if (q0 < groups) fetch(q0);
-        for (; q0 < groups; q0 += KS * 2) {
+        auto multiply = [&](int q0, const Step& x) {
             const int k0 = (q0 + (g >> 1)) * 256 + (g & 1) * 128;
-            v4u s[NB], z[NB];
-#pragma unroll
-            for (int j = 0; j < NB; j++) s[j] = sn[j], z[j] = zn[j];
-            if (q0 + KS * 2 < groups) fetch(q0 + KS * 2);
 #pragma unroll
             for (int d = 0; d < 4; d++) {
                 v4i e[MB], o[MB];
 #pragma unroll
                 for (int i = 0; i < MB; i++) {
-                    const v4i lo = token_piece(i, k0 + 32 * d), hi = token_piece(i, k0 + 32 * d + 16);
-                    uint32_t x[4], y[4];
-                    transpose_bytes({(uint32_t)lo[0], (uint32_t)lo[2], (uint32_t)hi[0], (uint32_t)hi[2]}, x);
-                    transpose_bytes({(uint32_t)lo[1], (uint32_t)lo[3], (uint32_t)hi[1], (uint32_t)hi[3]}, y);
-                    e[i] = v4i{(int)x[0], (int)x[1], (int)x[2], (int)x[3]}, o[i] = v4i{(int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+                    const v4i lo = TOKENS ? x.t[TOKENS ? 2 * d : 0] : token_piece(i, k0 + 32 * d), hi = TOKENS ? x.t[TOKENS ? 2 * d + 1 : 0] : token_piece(i, k0 + 32 * d + 16);
+                    uint32_t u[4], v[4];
+                    transpose_bytes({(uint32_t)lo[0], (uint32_t)lo[2], (uint32_t)hi[0], (uint32_t)hi[2]}, u);
+                    transpose_bytes({(uint32_t)lo[1], (uint32_t)lo[3], (uint32_t)hi[1], (uint32_t)hi[3]}, v);
+                    e[i] = v4i{(int)u[0], (int)u[1], (int)u[2], (int)u[3]}, o[i] = v4i{(int)v[0], (int)v[1], (int)v[2], (int)v[3]};
                 }
 #pragma unroll
                 for (int j = 0; j < NB; j++) {
                     uint32_t w[8];
-                    unpack32<W>(s[j][d], z[j][d], w);
+                    unpack32<W>(x.s[j][d], x.z[j][d], w);
                     const v4i w0 = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]}, w1 = {(int)w[4], (int)w[5], (int)w[6], (int)w[7]};
 #pragma unroll
                     for (int i = 0; i < MB; i++) {
@@ -289,6 +292,15 @@ __global__ __launch_bounds__(512) void k_i8_few(I8Product p, uint32_t ntiles) {
                     }
                 }
             }
+        };
+        Step now, next;
+        int q0 = wave * 2;
+        if (q0 < groups) fetch(q0, now);
+        for (; q0 < groups; q0 += KS * 4) {   // two steps, so that neither is copied
+            if (q0 + KS * 2 < groups) fetch(q0 + KS * 2, next);
+            multiply(q0, now);
+            if (q0 + KS * 4 < groups) fetch(q0 + KS * 4, now);
+            if (q0 + KS * 2 < groups) multiply(q0 + KS * 2, next);
         }
     }
     // accumulator e of a lane: weight row 4 g + e of its block, token r
@@ -359,15 +371,22 @@ template <I8Weights W>
 static hipError_t launch_few(I8Few f, int dtype, const I8Product& p, hipStream_t st) {
     return with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
-        auto run = [&](auto nb, auto mb) {
+        auto go = [&](auto nb, auto mb, auto few) {
             constexpr int NB = decltype(nb)::value, MB = decltype(mb)::value, bytes = 8 * 16 * MB * (16 * NB + 4) * 4;
             const int64_t ntiles = (p.N + 16 * NB - 1) / (16 * NB), tiles = ntiles * ((p.M + 16 * MB - 1) / (16 * MB));
             if (tiles > 0x7fffffff) return hipErrorInvalidConfiguration;
-            auto* const kern = k_i8_few<W, T, NB, MB>;
+            auto* const kern = k_i8_few<W, T, NB, MB, decltype(few)::value>;
             static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
             if (set != hipSuccess) return set;
             kern<<<dim3((unsigned)tiles), dim3(512), bytes, st>>>(p, (uint32_t)ntiles);
             return hipGetLastError();
+        };
+        // packed weights: a token's codes are asked for a step ahead up to four tokens; of more they fill the L1.  us, ahead / not: 1 x 16384 x 16384 18.0 / 21.7,
+        // 1 x 4096 x 14336 7.0 / 8.5, 16 x 16384 x 16384 26.6 / 23.9, 16 x 4096 x 4096 5.9 / 5.3
+        auto run = [&](auto nb, auto mb) {
+            if constexpr (W != I8Weights::Codes && decltype(mb)::value == 1)
+                if (p.M <= 4) return go(nb, mb, std::true_type{});
+            return go(nb, mb, std::false_type{});
         };
         using One = std::integral_constant<int, 1>;
         using Two = std::integral_constant<int, 2>;

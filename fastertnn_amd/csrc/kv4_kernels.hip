@@ -86,6 +86,18 @@ __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; i++) x[i] = (float)e[i];
 }
+// the same in two steps: as they lie, and as numbers
+template <typename T>
+struct Eight {
+    uint32_t w[2 * sizeof(T)];
+    __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(w, p, sizeof(w)); }
+    __device__ __forceinline__ void numbers(float (&x)[8]) const {
+        T e[8];
+        __builtin_memcpy(e, w, sizeof(w));
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (float)e[i];
+    }
+};
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
     T e[8];
@@ -94,55 +106,73 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
     __builtin_memcpy(p, e, sizeof(e));
 }
 
-// values d .. d + 7 of a row at position pos, rotated: products and sums in 64 bits, one rounding to fp32
-template <typename T>
-__device__ __forceinline__ void load_rotated(const T* row, int d, int pos, const Kv4Rotation& r, float (&y)[8]) {
-    load8(row + d, y);
+// cosines and sines of elements d .. d + 7 at a position, the sines with the sign of their term; what is not rotated has none
+struct Kv4Angles {
+    float c[8], n[8];
+};
+__device__ __forceinline__ void load_angles(const Kv4Rotation& r, int pos, int d, Kv4Angles& a) {
     if (d >= r.rot) return;
     const int half = r.rot / 2;
     const float *const c = r.cos + (int64_t)pos * half, *const n = r.sin + (int64_t)pos * half;
-    float other[8], cv[8], nv[8];
-    bool second[8];
-    if (r.neighbours && d + 8 <= r.rot) {   // whole pairs, four entries of the tables
+    if (r.neighbours && d + 8 <= r.rot) {   // whole pairs: four entries
         float c4[4], n4[4];
         __builtin_memcpy(c4, c + d / 2, 16), __builtin_memcpy(n4, n + d / 2, 16);
 #pragma unroll
-        for (int i = 0; i < 8; i++) other[i] = y[i ^ 1], cv[i] = c4[i / 2], nv[i] = n4[i / 2], second[i] = i & 1;
-    } else if (!r.neighbours && half % 8 == 0) {   // the other halves lie together
-        const bool late = d >= half;
-        const int at = late ? d - half : d;
-        load8(row + (late ? at : d + half), other);
-        __builtin_memcpy(cv, c + at, 32), __builtin_memcpy(nv, n + at, 32);
-#pragma unroll
-        for (int i = 0; i < 8; i++) second[i] = late;
+        for (int i = 0; i < 8; i++) a.c[i] = c4[i / 2], a.n[i] = n4[i / 2];
+    } else if (!r.neighbours && half % 8 == 0) {   // all of one half
+        const int at = d >= half ? d - half : d;
+        __builtin_memcpy(a.c, c + at, 32), __builtin_memcpy(a.n, n + at, 32);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const int e = min(d + i, r.rot - 1);   // (what is behind stays as it is)
-            second[i] = r.neighbours ? (e & 1) : e >= half;
-            const int at = r.neighbours ? e / 2 : second[i] ? e - half : e;
-            other[i] = r.neighbours ? y[i ^ 1] : (float)row[second[i] ? e - half : e + half];
-            cv[i] = c[at], nv[i] = n[at];
+            const int e = min(d + i, r.rot - 1), at = r.neighbours ? e / 2 : e >= half ? e - half : e;   // (what is behind stays as it is)
+            a.c[i] = c[at], a.n[i] = n[at];
         }
     }
 #pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (!(r.neighbours ? (i & 1) : d + i >= half)) a.n[i] = -a.n[i];
+}
+// values d .. d + 7 of a row and, where they are rotated, the other elements of their pairs
+template <typename T>
+__device__ __forceinline__ void load_pairs(const T* row, int d, const Kv4Rotation& r, Eight<T>& x, Eight<T>& other) {
+    x.load(row + d);
+    if (d >= r.rot || r.neighbours) return;   // (neighbours are among the eight)
+    const int half = r.rot / 2;
+    if (half % 8 == 0) {
+        other.load(row + (d >= half ? d - half : d + half));
+    } else {
+        T e[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int at = min(d + i, r.rot - 1);
+            e[i] = row[at >= half ? at - half : at + half];
+        }
+        __builtin_memcpy(other.w, e, sizeof(e));
+    }
+}
+// rotated: products and sums in 64 bits, one rounding to fp32
+__device__ __forceinline__ void rotate(const Kv4Rotation& r, int d, const Kv4Angles& a, float (&x)[8], const float (&other)[8]) {
+    if (d >= r.rot) return;
+    float y[8];
+#pragma unroll
     for (int i = 0; i < 8; i++) {
-        if (d + i >= r.rot) continue;
-        const double a = (double)y[i] * (double)cv[i], b = (double)other[i] * (double)nv[i];   // exact
-        other[i] = (float)(second[i] ? a + b : a - b);
+        const double q = (double)(r.neighbours ? x[i ^ 1] : other[i]) * (double)a.n[i];   // exact, as is the other product
+        y[i] = (float)__builtin_fma((double)x[i], (double)a.c[i], q);
     }
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        if (d + i < r.rot) y[i] = other[i];
-        asm volatile("" : "+v"(y[i]));   // in fp32 from here on: the compiler would make one rounding of this and a caller's to 16 bits
+        if (d + i < r.rot) x[i] = y[i];
+        asm volatile("" : "+v"(x[i]));   // in fp32 from here on: the compiler would make one rounding of this and a caller's to 16 bits
     }
 }
 
 // scale and zero of a group whose smallest and largest values are given, as the cache holds them: two bfloat16 in a word
-__device__ __forceinline__ uint32_t make_params(float low, float high, bool fine, float* scale, float* zero) {
-    const __bf16 z = (__bf16)low, s = (__bf16)(float)(((double)high - (double)low) / 15.0);
+__device__ __forceinline__ uint32_t make_params(float low, float high, float* scale, float* zero) {
+    // (times 1/15 in 64 bits: one rounding to fp32 is the quotient's)
+    const __bf16 z = (__bf16)low, s = (__bf16)(float)(((double)high - (double)low) * (1.0 / 15.0));
     *scale = (float)s, *zero = (float)z;
-    if (!fine || !(__builtin_fabsf(*zero) < __builtin_inff())) {
+    if (!(__builtin_fabsf(*zero) < __builtin_inff())) {   // of a group with a NaN or an infinity, or a zero beyond bfloat16
         *scale = *zero = __builtin_nanf("");
         return 0x7FC07FC0u;
     }
@@ -151,20 +181,24 @@ __device__ __forceinline__ uint32_t make_params(float low, float high, bool fine
 __device__ __forceinline__ float scale_of(uint32_t params) { return __builtin_bit_cast(float, params << 16); }
 __device__ __forceinline__ float zero_of(uint32_t params) { return __builtin_bit_cast(float, params & 0xFFFF0000u); }
 
-// Eight codes.  A difference, a reciprocal and a product in fp32 are off by less than 4 * 2^-24 of a quotient of up to 16, 2^-18: where none of the eight is
-// within 2^-16 of a border between codes they are what the formula says.  Others are divided in 64 bits.
-__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float scale, float zero) {
+// Eight codes.  A difference, the reciprocal and a product in fp32 are off by at most (2^-24 + 2^-23 + 2^-24) of a quotient of up to 16, 2^-18: where none of
+// the eight is within 2^-16 of a border between codes they are what the formula says.  Others are divided in 64 bits.  Adding 1.5 * 2^23 rounds to a whole
+// number, ties to even, which is the lowest bits of the sum; the bits of the constant, moved along, are taken off at the end.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float scale, float zero, float high) {
     if (!(scale > 0.0f)) return 0;
-    const float inv = 1.0f / scale;
+    constexpr uint32_t kBits = 0x4B400000u;
+    constexpr uint32_t kOnes = 0x11111111u;   // sum of 16^e
+    const float inv = __builtin_amdgcn_rcpf(scale);
     uint32_t w = 0;
-    bool near = !(inv < __builtin_inff());
+    float far = 0.0f;   // the largest distance from a whole number
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        const float q = (x[e] - zero) * inv, n = __builtin_rintf(q);
-        near |= !(q <= 17.0f) || __builtin_fabsf(__builtin_fabsf(q - n) - 0.5f) < 0x1p-16f;   // (more than 17: the difference is beyond fp32)
-        w |= (uint32_t)__builtin_fminf(__builtin_fmaxf(n, 0.0f), 15.0f) << (4 * e);
+        const float q = __builtin_amdgcn_fmed3f((x[e] - zero) * inv, 0.0f, 15.0f), t = q + 12582912.0f;
+        far = fmaxf(far, __builtin_fabsf(q - (t - 12582912.0f)));
+        w += __builtin_bit_cast(uint32_t, t) << (4 * e);
     }
-    if (near) {
+    w -= kBits * kOnes;
+    if (far > 0.5f - 0x1p-16f || scale < 0x1p-100f || !(high - zero < __builtin_inff())) {   // (a difference beyond fp32, a scale without a reciprocal)
         w = 0;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
@@ -175,25 +209,44 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float scale, f
     return w;
 }
 
-template <int LG>
-__device__ __forceinline__ void group_range(const float (&y)[8], bool live, float* low, float* high, bool* fine) {
-    float lo = __builtin_inff(), hi = -__builtin_inff();
-    int ok = 1;
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (live) {
-            lo = fminf(lo, y[i]), hi = fmaxf(hi, y[i]);
-            ok &= __builtin_fabsf(y[i]) < __builtin_inff() ? 1 : 0;
-        }
-#pragma unroll
-    for (int d = 1; d < LG; d *= 2) {
-        lo = fminf(lo, __shfl_xor(lo, d)), hi = fmaxf(hi, __shfl_xor(hi, d));
-        ok &= __shfl_xor(ok, d);
+// lane i and the lane that differs from it in bit B alone, once all lower bits agree: exchanged in the vector ALU
+template <int B>
+__device__ __forceinline__ float across(float x) {
+    const int v = __builtin_bit_cast(int, x);
+    if constexpr (B == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+        return __builtin_bit_cast(float, (uint32_t)((lane_id() & 16) ? r[0] : r[1]));
+    } else {
+        // quad_perm [1,0,3,2], quad_perm [2,3,0,1], row_half_mirror, row_mirror
+        constexpr int ctrl = B == 1 ? 0xB1 : B == 2 ? 0x4E : B == 4 ? 0x141 : 0x140;
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, v, ctrl, 0xF, 0xF, false));
     }
-    *low = lo, *high = hi, *fine = ok;
 }
 
-// One wavefront per (block of 8 positions, head): four heads of keys and values, and behind those of queries, per workgroup.  LG lanes hold a token's
+// smallest and largest value of the LG lanes that hold a token; of one with a NaN or an infinity the smallest is -infinity
+template <int LG>
+__device__ __forceinline__ void group_range(const float (&y)[8], bool live, float* low, float* high) {
+    float lo = __builtin_inff(), hi = -__builtin_inff();
+    if (live) {
+        float none = 0.0f;   // 0 times a NaN or an infinity is a NaN
+        lo = hi = y[0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) lo = fminf(lo, y[i]), hi = fmaxf(hi, y[i]);
+#pragma unroll
+        for (int i = 0; i < 8; i++) none = __builtin_fmaf(y[i], 0.0f, none);
+        lo = none == 0.0f ? lo : -__builtin_inff();
+    }
+    auto step = [&](float l, float h) { lo = fminf(lo, l), hi = fmaxf(hi, h); };
+    step(across<1>(lo), across<1>(hi));
+    step(across<2>(lo), across<2>(hi));
+    step(across<4>(lo), across<4>(hi));
+    if constexpr (LG > 8) step(across<8>(lo), across<8>(hi));
+    if constexpr (LG > 16) step(across<16>(lo), across<16>(hi));
+    *low = lo, *high = hi;
+}
+
+// A wavefront per (block of 8 positions, head of keys and values, or behind those of queries); where there are many it takes one head after the other, so
+// that finding the block is paid once for several.  LG lanes hold a token's
 // channels, eight each.  The codes of a block's values meet in LDS, where every lane makes the words of its channels; what the block holds already of
 // other tokens stays.
 template <typename T, int D>
@@ -201,67 +254,96 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4 kv, Kv4Rows k, Kv4Rows v
     constexpr int LG = D <= 64 ? 8 : D <= 128 ? 16 : 32, TPI = 64 / LG;   // lanes of a token, tokens at a time
     __shared__ uint32_t codes[4][8][D / 8];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane % LG, d = 8 * li;
-    int head = blockIdx.y * 4 + wave;
-    if (head >= kv.heads + heads_q) return;   // (nothing below waits for another wavefront)
     const Kv4Eight at = find_eight(kv, blockIdx.x);
     const int count = r.rot ? min(at.count, r.positions - at.pos) : at.count;
     if (count <= 0 || at.pos < 0) return;
-    if (head >= kv.heads) {
-        head -= kv.heads;
-#pragma unroll
-        for (int i0 = 0; i0 < 8; i0 += TPI) {
-            const int i = i0 + lane / LG;
-            if (i < count && d < D) {
-                float y[8];
-                load_rotated(static_cast<const T*>(q.p) + (at.t + i) * q.token_stride + head * q.head_stride, d, at.pos + i, r, y);
-                store8(q_out + ((int64_t)(at.t + i) * heads_q + head) * D + d, y);
-            }
-        }
-        return;
-    }
     const int64_t id = kv.page_of(at.s, at.pos);
-    if (id < 0) return;
-    char* const block = kv.block(id, head);
-    const int slot = at.pos & (kv.page - 1);
+    const int slot = at.pos & (kv.page - 1), place = slot & 7;
+    constexpr int JS = 8 / TPI;
+    Kv4Angles angles[JS];   // of the lane's channels: the same for all heads
 #pragma unroll
-    for (int which = 0; which < 2; which++) {
-        float y[8 / TPI][8];   // all of the block is asked for at once
+    for (int j = 0; j < JS; j++) {
+        const int i = j * TPI + lane / LG;
+        if (i < count && d < D) load_angles(r, at.pos + i, d, angles[j]);
+    }
+    // a head's rows of the block, all asked for at once
+    struct Rows {
+        Eight<T> x[JS], other[JS], value[JS];
+    };
+    const int heads = kv.heads + heads_q, step = 4 * gridDim.y;
+    auto fetch = [&](int head, Rows& rows) {
+        const bool query = head >= kv.heads;
+        const T* const from = query ? static_cast<const T*>(q.p) + at.t * q.token_stride + (head - kv.heads) * q.head_stride
+                                    : static_cast<const T*>(k.p) + at.t * k.token_stride + head * k.head_stride;
+        const T* const values = static_cast<const T*>(v.p) + at.t * v.token_stride + head * v.head_stride;
+        const int64_t stride = query ? q.token_stride : k.token_stride;
 #pragma unroll
-        for (int j = 0; j < 8 / TPI; j++) {
+        for (int j = 0; j < JS; j++) {
             const int i = j * TPI + lane / LG;
             if (i < count && d < D) {
-                if (which == 0) load_rotated(static_cast<const T*>(k.p) + (at.t + i) * k.token_stride + head * k.head_stride, d, at.pos + i, r, y[j]);
-                else load8(static_cast<const T*>(v.p) + (at.t + i) * v.token_stride + head * v.head_stride + d, y[j]);
+                load_pairs(from + i * stride, d, r, rows.x[j], rows.other[j]);
+                if (!query) rows.value[j].load(values + i * v.token_stride + d);
             }
         }
+    };
+    for (int head = blockIdx.y * 4 + wave; head < heads; head += step) {   // (no wavefront waits for another)
+        Rows rows;
+        fetch(head, rows);
 #pragma unroll
-        for (int j = 0; j < 8 / TPI; j++) {
-            if (j * TPI >= count) break;
-            const int i = j * TPI + lane / LG;
-            const bool live = i < count && d < D;
-            float low, high, scale, zero;
-            bool fine;
-            group_range<LG>(y[j], live, &low, &high, &fine);
-            const uint32_t params = make_params(low, high, fine, &scale, &zero);
-            if (live) {
-                const uint32_t w = codes_of(y[j], scale, zero);
-                if (which == 0) *reinterpret_cast<uint32_t*>(block + (slot + i) * (D / 2) + d / 2) = w;
-                else codes[wave][i][li] = w;
-                if (li == 0) *reinterpret_cast<uint32_t*>(block + (which ? kv.value_params() : kv.key_params()) + (slot + i) * 4) = params;
+        for (int j = 0; j < JS; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) asm volatile("" : "+v"(angles[j].c[e]), "+v"(angles[j].n[e]));   // (kept in 32 bits between heads)
+        const bool query = head >= kv.heads;
+        if (!query && id < 0) continue;
+        float y[JS][8];
+#pragma unroll
+        for (int j = 0; j < JS; j++) {
+            float other[8];
+            rows.x[j].numbers(y[j]), rows.other[j].numbers(other);
+            rotate(r, d, angles[j], y[j], other);
+        }
+        if (query) {
+#pragma unroll
+            for (int j = 0; j < JS; j++) {
+                const int i = j * TPI + lane / LG;
+                if (i < count && d < D) store8(q_out + ((int64_t)(at.t + i) * heads_q + head - kv.heads) * D + d, y[j]);
+            }
+            continue;
+        }
+        char* const block = kv.block(id, head);
+#pragma unroll
+        for (int which = 0; which < 2; which++) {
+#pragma unroll
+            for (int j = 0; j < JS; j++)
+                if (which == 1) rows.value[j].numbers(y[j]);
+#pragma unroll
+            for (int j = 0; j < JS; j++) {
+                if (j * TPI >= count) break;
+                const int i = j * TPI + lane / LG;
+                const bool live = i < count && d < D;
+                float low, high, scale, zero;
+                group_range<LG>(y[j], live, &low, &high);
+                const uint32_t params = make_params(low, high, &scale, &zero);
+                if (live) {
+                    const uint32_t w = codes_of(y[j], scale, zero, high);
+                    if (which == 0) *reinterpret_cast<uint32_t*>(block + (slot + i) * (D / 2) + d / 2) = w;
+                    else codes[wave][i][li] = w;
+                    if (li == 0) *reinterpret_cast<uint32_t*>(block + (which ? kv.value_params() : kv.key_params()) + (slot + i) * 4) = params;
+                }
             }
         }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // the wavefront's own codes: its LDS accesses keep their order
-    __builtin_amdgcn_wave_barrier();
-    uint32_t* const words = reinterpret_cast<uint32_t*>(block + kv.values()) + (slot / 8) * D;
-    const int place = slot & 7;
-    for (int e = lane; e < D; e += 64) {
-        uint32_t w = 0;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // the wavefront's own codes: its LDS accesses keep their order
+        __builtin_amdgcn_wave_barrier();
+        uint32_t* const words = reinterpret_cast<uint32_t*>(block + kv.values()) + (slot / 8) * D;
+        for (int e = lane; e < D; e += 64) {
+            uint32_t w = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i < count) w |= (codes[wave][i][e / 8] >> (4 * (e & 7)) & 15u) << (4 * (place + i));
-        if (count < 8) w |= words[e] & ~((0xFFFFFFFFu >> (32 - 4 * count)) << (4 * place));
-        words[e] = w;
+            for (int i = 0; i < 8; i++)
+                if (i < count) w |= (codes[wave][i][e / 8] >> (4 * (e & 7)) & 15u) << (4 * (place + i));
+            if (count < 8) w |= words[e] & ~((0xFFFFFFFFu >> (32 - 4 * count)) << (4 * place));
+            words[e] = w;
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -837,10 +919,12 @@ Kv4Plan plan_of(const ftnn_kv4_t& kv, int heads_q, int max_len) {
 hipError_t launch_kv4_append(const ftnn_kv4_t& kv, int dtype, const Kv4Rows& k, const Kv4Rows& v, const Kv4Rotation& r, int heads_q,
                              const Kv4Rows& q, void* d_q_out, hipStream_t st) {
     const Kv4 dv = device_view(kv);
+    const int eights = eights_of(kv), groups = (kv.heads + heads_q + 3) / 4;
+    const int heads_at_a_time = std::max(1, std::min(groups, (512 + eights - 1) / eights));   // about two workgroups per compute unit, or all there are
     return with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
         return with_dim(kv.dim, [&](auto d) {
-            k_kv4_append<T, decltype(d)::value><<<dim3(eights_of(kv), (kv.heads + heads_q + 3) / 4), dim3(256), 0, st>>>(dv, k, v, r, heads_q, q, static_cast<T*>(d_q_out));
+            k_kv4_append<T, decltype(d)::value><<<dim3(eights, heads_at_a_time), dim3(256), 0, st>>>(dv, k, v, r, heads_q, q, static_cast<T*>(d_q_out));
             return hipGetLastError();
         });
     });
