@@ -795,30 +795,35 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT, D * CB <= 256 && D < 256 ?
         const int64_t all = (int64_t)kv.tokens * p.heads_q;
         const float* const ml = lds + WT * TILE * LD;
         __syncthreads();
-        for (int x = threadIdx.x; x < TILE * D; x += 64 * WT) {
-            const int r = x / D, d = x % D;
-            const uint32_t rr = row0 + r;
-            if (rr >= rows) break;
-            float top = -__builtin_inff(), sum = 0.0f, den = 0.0f;
+        // 16 lanes to a row, NB channels each
+        const int r = threadIdx.x >> 4, d = (threadIdx.x & 15) * NB;
+        static_assert(WT * 64 == 16 * TILE, "a lane per NB channels of the tile");
+        const uint32_t rr = row0 + r;
+        if (rr >= rows) return;
+        float top = -__builtin_inff(), den = 0.0f, f[WT], sum[NB] = {};
 #pragma unroll
-            for (int w = 0; w < WT; w++) top = fmaxf(top, ml[(w * TILE + r) * 2]);
-            const float safe = top == -__builtin_inff() ? 0.0f : top;
+        for (int w = 0; w < WT; w++) top = fmaxf(top, ml[(w * TILE + r) * 2]);
 #pragma unroll
-            for (int w = 0; w < WT; w++) {
-                const float lw = ml[(w * TILE + r) * 2 + 1];
-                const float f = lw == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[(w * TILE + r) * 2] - safe);
-                sum = __builtin_fmaf(lds[(w * TILE + r) * LD + d], f, sum);
-                den = __builtin_fmaf(lw, f, den);
-            }
-            const int64_t at = row_at(rr);
-            if (p.splits == 1) {
-                static_cast<T*>(p.out)[at * D + d] = (T)(den == 0.0f ? 0.0f : sum / den);
-            } else {
-                p.part[(split * all + at) * D + d] = sum;
-                if (d == 0) {
-                    float* const pm = p.part + p.splits * all * D + (split * all + at) * 2;
-                    pm[0] = top, pm[1] = den;
-                }
+        for (int w = 0; w < WT; w++) {
+            const float lw = ml[(w * TILE + r) * 2 + 1];
+            f[w] = lw == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[(w * TILE + r) * 2] - top);   // (sums without weights are zeros)
+            den = __builtin_fmaf(lw, f[w], den);
+        }
+#pragma unroll
+        for (int w = 0; w < WT; w++)
+#pragma unroll
+            for (int i = 0; i < NB; i++) sum[i] = __builtin_fmaf(lds[(w * TILE + r) * LD + d + i], f[w], sum[i]);
+        const int64_t at = row_at(rr);
+        if (p.splits == 1) {
+            T y[NB];
+#pragma unroll
+            for (int i = 0; i < NB; i++) y[i] = (T)(den == 0.0f ? 0.0f : sum[i] / den);
+            __builtin_memcpy(static_cast<T*>(p.out) + at * D + d, y, sizeof(y));
+        } else {
+            __builtin_memcpy(p.part + (split * all + at) * D + d, sum, sizeof(sum));
+            if (d == 0) {
+                float* const pm = p.part + p.splits * all * D + (split * all + at) * 2;
+                pm[0] = top, pm[1] = den;
             }
         }
     }
@@ -890,10 +895,11 @@ hipError_t with_dim(int dim, F&& fn) {
     }
 }
 
-// How a call is split.  Tiles of 16 rows, whose tokens the four wavefronts of a workgroup share, or, where that fills the chip, wavefronts of 32 rows (16
-// of dim 256) on all tokens: they read and unpack the cache once for twice the rows and have no partial sums to join.  Fewer workgroups than
-// run at once (two per compute unit, one of dim 256) split their tokens further, down to 512 each, and a second launch joins the parts.  us, 16 / 32 rows,
-// 8 heads of 4 x 128 at a length of 4000: 512 new tokens 83 / 102, 1024 156 / 187, 2048 247 / 217; 4 x 512 at 2000 126 / 109.
+// How a call is split: tiles of 16 rows, whose tokens the four wavefronts of a workgroup share, or wavefronts of 32 rows (16 of dim 256) on all tokens, which
+// read and unpack the cache once for twice the rows and have no sums to join.  Fewer workgroups of the first kind than run at once (two per compute
+// unit, one of dim 256) split their tokens further, down to 512 each, and a second launch joins the parts.  The choice goes by an estimate in us: a workgroup
+// costs 6 and a step of 32 tokens of a wavefront `narrow` or `wide`; fitted to 8 heads of 4 x 128 at 4000 tokens, 16 / 32 rows measured: 512 new 83 / 167,
+// 1024 156 / 186, 2048 247 / 217, 4 x 512 at 2000 126 / 109, 512 at 512 23.5 / 25.9; of dim 256, 4 heads: 1000 new 174 / 184.
 struct Kv4Plan {
     int blocks, waves;   // CB, WT
     int64_t tiles;
@@ -904,14 +910,18 @@ int64_t tiles_of(const ftnn_kv4_t& kv, int group, int rows) {   // at most: toke
     return std::min((t * group + rows - 1) / rows + kv.sequences, t * ((group + rows - 1) / rows));
 }
 Kv4Plan plan_of(const ftnn_kv4_t& kv, int heads_q, int max_len) {
-    const int group = heads_q / kv.heads;
+    const int group = heads_q / kv.heads, blocks = kv.dim <= 128 ? 2 : 1;
     const int64_t capacity = (int64_t)kv.width * kv.page, most = max_len > 0 ? std::min<int64_t>(max_len, capacity) : capacity;
-    const int64_t resident = kv.dim == 256 ? 240 : 512, least = 512;
-    auto splits = [&](int64_t tiles) { return (int)std::max<int64_t>(1, std::min<int64_t>({resident / std::max<int64_t>(1, tiles * kv.heads), (most + least - 1) / least, kMostSplits})); };
-    const int blocks = kv.dim <= 128 ? 2 : 1;
-    const int64_t wide = tiles_of(kv, group, 64 * blocks), narrow = tiles_of(kv, group, 16);
-    if ((int64_t)kv.tokens * group / (64 * blocks) * kv.heads >= 480) return {blocks, 1, wide, 1};
-    return {1, 4, narrow, splits(narrow)};
+    const int64_t resident = kv.dim == 256 ? 240 : 512;
+    const int64_t wide = tiles_of(kv, group, 64 * blocks), narrow = tiles_of(kv, group, 16), spread = std::max<int64_t>(1, narrow * kv.heads);
+    const int splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident / spread, (most + 511) / 512, kMostSplits}));
+    const double narrow_step = kv.dim == 64 ? 0.8 : kv.dim <= 128 ? 1.1 : 1.2, wide_step = kv.dim == 64 ? 1.2 : kv.dim <= 128 ? 1.6 : 1.45;
+    const double steps = std::max(1.0, ((double)most - 0.5 * kv.tokens / std::max(kv.sequences, 1)) / 32);   // of a row, in the mean
+    auto rounds = [&](int64_t workgroups, int64_t at_once) { return (double)((workgroups + at_once - 1) / at_once); };
+    const double by16 = rounds(spread * splits, resident) * (6 + std::max(1.0, steps / 4 / splits) * narrow_step) + (splits > 1 ? 5 : 0);
+    const double by32 = rounds(wide * kv.heads, 512) * (6 + steps * wide_step);
+    if (by32 < by16) return {blocks, 1, wide, 1};
+    return {1, 4, narrow, splits};
 }
 
 }  // namespace
