@@ -11,4 +11,6 @@ TILES = {
 }
 # (nb, mb): (m, n) for codes and for packed rows
 FEW_CODES = {(1, 1): (33, 1000), (1, 2): (50, 2001), (2, 1): (9, 8001)}
-FEW_PACKED = {(1, 1): (33, 1000), (2, 1): (20, 4500), (4, 1): (15, 21001), (4, 2): (32, 11003), (4, 4): (200, 5003)}
+FEW_PACKED = {(1, 1): (33, 1000), (2, 1): (20, 4500), (4, 1): (15, 21001), (4, 2): (32, 11003), (4, 4): (200, 4003)}
+FEW_K = (16, 1025, 5000)   # lengths of a row at which the packed ones have their form
+TILES_PACKED = ("T256", "T128Two")   # those of the above whose longest rows run as tiles when packed

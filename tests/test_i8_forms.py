@@ -24,7 +24,7 @@ int main() {
     long long m, n;
     int packed, k;
     while (scanf("%d %lld %lld %d", &packed, &m, &n, &k) == 4) {
-        const ftnn::I8Few f = ftnn::i8_few(packed, m, n);
+        const ftnn::I8Few f = ftnn::i8_few(packed, m, n, k);
         printf("%d %d %d\n", f.nb, f.mb, (int)ftnn::i8_form(m, n, k));
     }
 }
@@ -43,10 +43,14 @@ def test_shapes_of_the_gpu_tests(choose):
     for name, ((m, n), ks) in i8_shapes.TILES.items():
         assert choose([(0, m, n, k) for k in ks]) == [((0, 0), name)] * len(ks)
         assert [f[1] for f in choose([(1, m, n, k) for k in ks])] == [name] * len(ks)
+    for name in i8_shapes.TILES_PACKED:
+        (m, n), ks = i8_shapes.TILES[name]
+        assert choose([(1, m, n, ks[-1])]) == [((0, 0), name)]
     for packed, table in ((0, i8_shapes.FEW_CODES), (1, i8_shapes.FEW_PACKED)):
         for form, (m, n) in table.items():
-            assert choose([(packed, m, n, 100)])[0][0] == form
-            assert not packed or lib.mm_i8_rows_scratch_bytes(True, m, n, 100) == 0
+            for k in i8_shapes.FEW_K:
+                assert choose([(packed, m, n, k)])[0][0] == form
+                assert not packed or lib.mm_i8_rows_scratch_bytes(True, m, n, k) == 0
 
 
 def test_every_size_has_a_form(choose):
