@@ -47,17 +47,19 @@ struct TileOrder {
     }
 };
 
-template <int WM, int WN, int NS, int BK, int KG>
+constexpr int BK = 128;   // codes of a step
+
+template <int WM, int WN, int NS, int KG>
 struct TileShape {
     static constexpr int RPL = 1024 / BK, PPR = BK / 16;   // rows of a load, pieces of a row
     static constexpr int TM = 64 * WM, TN = 64 * WN, STAGE = (TM + TN) * BK, FM = TM / (4 * RPL), FN = TN / (4 * RPL), FW = FM + FN;
-    static __device__ __forceinline__ int swizzle(int r) { return BK == 128 ? r & 7 : r >> 1 & 3; }
+    static __device__ __forceinline__ int swizzle(int r) { return r & (PPR - 1); }
     static constexpr int ring = NS * STAGE, lds = KG * ring + (TM + 2 * TN) * 4;   // a ring per group, and the tile's scales and bias
 };
 
-template <typename T, int WM, int WN, int NS, int BK, int KG>
+template <typename T, int WM, int WN, int NS, int KG>
 __global__ __launch_bounds__(256 * KG) void k_i8_tiles(I8Product p, TileOrder order) {
-    typedef TileShape<WM, WN, NS, BK, KG> TS;
+    typedef TileShape<WM, WN, NS, KG> TS;
     constexpr int TM = TS::TM, TN = TS::TN, FM = TS::FM, FN = TS::FN, FW = TS::FW, NL = WM + WN, NM = WM * WN;
     extern __shared__ __align__(16) int8_t all_lds[];
     const int lane = threadIdx.x & 63, group = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
@@ -252,10 +254,10 @@ __global__ __launch_bounds__(256 * KG) void k_i8_tiles(I8Product p, TileOrder or
     }
 }
 
-template <typename T, int WM, int WN, int NS, int BK, int KG>
+template <typename T, int WM, int WN, int NS, int KG>
 hipError_t launch(const I8Product& p, hipStream_t st) {
-    typedef TileShape<WM, WN, NS, BK, KG> TS;
-    auto* const kern = k_i8_tiles<T, WM, WN, NS, BK, KG>;
+    typedef TileShape<WM, WN, NS, KG> TS;
+    auto* const kern = k_i8_tiles<T, WM, WN, NS, KG>;
     static const hipError_t configured = [&]() {
         hipFuncAttributes attr;   // a scratch access would move the count that the waits rely on
         hipError_t e = hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(kern));
@@ -278,12 +280,12 @@ hipError_t launch_i8_tiles(int dtype, const I8Product& p, hipStream_t st) {
     return with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
         switch (i8_form(p.M, p.N, p.K)) {
-            case I8Form::T256: return launch<T, 4, 4, 2, 128, 1>(p, st);
-            case I8Form::T128: return launch<T, 2, 2, 4, 128, 1>(p, st);
-            case I8Form::T128Two: return launch<T, 2, 2, 2, 128, 1>(p, st);
-            case I8Form::T128x64: return launch<T, 2, 1, 3, 128, 1>(p, st);
-            case I8Form::T64: return launch<T, 1, 1, 4, 128, 1>(p, st);
-            default: return launch<T, 1, 1, 4, 128, 2>(p, st);
+            case I8Form::T256: return launch<T, 4, 4, 2, 1>(p, st);
+            case I8Form::T128: return launch<T, 2, 2, 4, 1>(p, st);
+            case I8Form::T128Two: return launch<T, 2, 2, 2, 1>(p, st);
+            case I8Form::T128x64: return launch<T, 2, 1, 3, 1>(p, st);
+            case I8Form::T64: return launch<T, 1, 1, 4, 1>(p, st);
+            default: return launch<T, 1, 1, 4, 2>(p, st);
         }
     });
 }

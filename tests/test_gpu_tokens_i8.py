@@ -25,7 +25,7 @@ def _same_codes(x, q, scale):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,k", [(1, 1), (3, 15), (1, 16), (5, 17), (2, 100), (70, 257), (4, 1024), (9, 4100), (2, 16384), (1, 16387), (3, 40001)])
+@pytest.mark.parametrize("rows,k", [(1, 1), (3, 15), (1, 16), (5, 17), (2, 100), (70, 257), (7, 512), (5, 520), (4, 1024), (6, 1040), (13, 2048), (3, 2049), (9, 4100), (2, 16384), (1, 16387), (3, 40001)])
 def test_codes_of_rows(dtype, rows, k):
     x = _rand(rows * 1000 + k, (rows, k), TYPES[dtype])
     _same_codes(x, *lib.quantize_rows_i8(x.cuda()))
