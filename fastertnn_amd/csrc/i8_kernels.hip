@@ -23,7 +23,7 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 // multiply-add issues at the rate of a 32-bit one, so this costs three instructions per value beside the loads.
 //
 // A row is read once: its values stay in registers between the maximum and the codes, up to NV vectors of 16 bytes per thread; what
-// is beyond that is read again.
+// is beyond that is read again, mostly from the L2.  Memory bounds it: 8192 x 11007 float32 109 us, 4.1 TB/s of what has to move (a copy: 5.07).
 
 template <typename T>
 struct Vec {   // 16 bytes of T
@@ -184,7 +184,9 @@ __device__ __forceinline__ void unpack32(uint32_t s, uint32_t z, uint32_t (&out)
 }
 
 // Few tokens: KS wavefronts split K over one tile of 16 NB weight rows x 16 MB tokens and meet in LDS.  Operands come straight from memory
-// into registers, the next step's while this one is multiplied.
+// into registers, the next step's while this one is multiplied.  What a compute unit can have on its way through its L1 bounds codes (17 bytes per clock; two,
+// three or four steps ahead are no faster than one), 1 x 4096 x 4096 6.1 us with its launch; packed weights are bounded by memory for one token (16384 x 16384
+// ternary 17.6 us, 3.8 TB/s) and by unpacking, 4 instructions per word of codes, for many.
 template <I8Weights W, typename T, int NB, int MB, bool TOKENS>
 __global__ __launch_bounds__(512) void k_i8_few(I8Product p, uint32_t ntiles) {
     constexpr int KS = 8, LD = 16 * NB + 4;
@@ -342,7 +344,7 @@ __global__ __launch_bounds__(512) void k_i8_few(I8Product p, uint32_t ntiles) {
     }
 }
 
-// packed rows -> rows of codes, 32 lanes per thread
+// packed rows -> rows of codes, 32 lanes per thread; stores bound it: 5003 x 4100 in 5 us
 template <I8Weights W>
 __global__ __launch_bounds__(256) void k_unpack_rows(const uint32_t* __restrict__ B, int64_t N, int K, int8_t* __restrict__ out, int64_t stride) {
     constexpr bool TERN = W == I8Weights::Ternary;
@@ -366,16 +368,22 @@ hipError_t launch_quantize_rows_i8(int dtype, const void* d_x, int64_t x_stride,
                                    float* d_scale, hipStream_t st) {
     return with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
-        const T* const x = static_cast<const T*>(d_x);
         // A wavefront per row where it holds the row in four vectors a lane (or in one, which leaves more of them at a time), else a workgroup.  us,
         // workgroup / wavefront of four / of one, bf16: 65536 x 128 72.4 / 26.2 / 19.3, 16384 x 512 20.8 / 9.2 / 7.6, 4096 x 2048 9.0 / 7.4 / 7.7,
         // 4096 x 4096 11.4 / 12.4 / 13.1, 8192 x 8192 33.7 / 51.7 / 57.2; few rows alike
         const int nvec = ((K + 15) / 16) * 16 / Vec<T>::N;
-        const dim3 four((unsigned)((rows + 3) / 4));
-        if (nvec <= 64) k_quantize_rows<T, 1, 4, 1><<<four, dim3(256), 0, st>>>(x, x_stride, rows, K, d_q, q_stride, d_scale);
-        else if (nvec <= 256) k_quantize_rows<T, 1, 4, 4><<<four, dim3(256), 0, st>>>(x, x_stride, rows, K, d_q, q_stride, d_scale);
-        else k_quantize_rows<T, 4, 1, 4><<<dim3((unsigned)rows), dim3(256), 0, st>>>(x, x_stride, rows, K, d_q, q_stride, d_scale);
-        return hipGetLastError();
+        constexpr int64_t kRows = 1 << 23;   // of a launch, which holds fewer than 2^32 threads
+        for (int64_t r = 0; r < rows; r += kRows) {
+            const int64_t n = std::min(rows - r, kRows);
+            const T* const x = static_cast<const T*>(d_x) + r * x_stride;
+            const dim3 four((unsigned)((n + 3) / 4));
+            if (nvec <= 64) k_quantize_rows<T, 1, 4, 1><<<four, dim3(256), 0, st>>>(x, x_stride, n, K, d_q + r * q_stride, q_stride, d_scale + r);
+            else if (nvec <= 256) k_quantize_rows<T, 1, 4, 4><<<four, dim3(256), 0, st>>>(x, x_stride, n, K, d_q + r * q_stride, q_stride, d_scale + r);
+            else k_quantize_rows<T, 4, 1, 4><<<dim3((unsigned)n), dim3(256), 0, st>>>(x, x_stride, n, K, d_q + r * q_stride, q_stride, d_scale + r);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+        return hipSuccess;
     });
 }
 
@@ -400,7 +408,7 @@ static hipError_t launch_few(I8Few f, int dtype, const I8Product& p, hipStream_t
         auto go = [&](auto nb, auto mb, auto few) {
             constexpr int NB = decltype(nb)::value, MB = decltype(mb)::value, bytes = 8 * 16 * MB * (16 * NB + 4) * 4;
             const int64_t ntiles = (p.N + 16 * NB - 1) / (16 * NB), tiles = ntiles * ((p.M + 16 * MB - 1) / (16 * MB));
-            if (tiles > 0x7fffffff) return hipErrorInvalidConfiguration;
+            if (tiles >= 1 << 23) return hipErrorInvalidConfiguration;   // a launch holds fewer than 2^32 threads
             auto* const kern = k_i8_few<W, T, NB, MB, decltype(few)::value>;
             static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
             if (set != hipSuccess) return set;

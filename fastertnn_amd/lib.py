@@ -585,11 +585,11 @@ def kv4_attention(q, cache, table, lens, starts, heads, page, scale=None, max_le
     """ftnn_kv4_attention: queries [tokens][heads_q][dim] of the new tokens over what the cache holds of their sequences, each token
     seeing itself and those before it; scale defaults to dim ** -0.5.  Rows of no sequence are left as they are in out (not set in one
     that is made here)."""
-    r = (_call or _native()).kv4_attention(cache, table, lens, starts, q, heads, page, q.shape[-1] ** -0.5 if scale is None else scale, max_len, out, scratch)
+    _need(q.dim() == 3 and q.shape[2] > 0, "q: expected tokens, heads and channels, got shape %s", tuple(q.shape))
+    r = (_call or _native()).kv4_attention(cache, table, lens, starts, q, heads, page, q.shape[2] ** -0.5 if scale is None else scale, max_len, out, scratch)
     if r is not None:
         return _given(r)
     t = torch or _torch()
-    _need(q.dim() == 3, "q: expected 3 dimensions, got %d", q.dim())
     tokens, heads_q, dim = q.shape
     d = _kv4(cache, table, lens, starts, tokens, heads, dim, page)
     qp = _token_rows(q, "q", q.dtype, tokens, dim)

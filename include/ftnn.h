@@ -385,7 +385,8 @@ FTNN_API int ftnn_quantize_rows_i8(int dtype, const void *d_x, int64_t x_stride,
  * y[m][n] = sum_k a[m][k] b[n][k] * sa[m] * sb[n] + bias[n], sums in 32-bit integers, scales applied in fp32 in that order, one
  * rounding to the result's type.  d_a, d_b: rows of 8-bit codes as above (16-byte aligned, strides multiples of 16; the bytes from K up to
  * ftnn_i8_row_bytes(K) are zero in one of the two).  d_bias may be NULL.  d_y: rows of N values, y_stride values apart.  K at
- * most 131071 (32-bit sums of any codes); M and N below 2^31, M * N below 2^40.
+ * most 131071 (32-bit sums of any codes); M and N below 2^31, M * N below 2^40 (and 2^23 tiles, of 16 x 16 results at least: FTNN_EHIP
+ * beyond).
  */
 FTNN_API int ftnn_mm_i8(int dtype, const int8_t *d_a, int64_t a_stride, const float *d_sa, const int8_t *d_b,
                         int64_t b_stride, const float *d_sb, const float *d_bias, int64_t M, int64_t N, int K, void *d_y,

@@ -232,6 +232,46 @@ def test_on_streams_and_in_graphs():
         assert torch.equal(y, step())
 
 
+def test_two_graphs_of_packed_products():
+    """tiles behind the launch that unpacks: two captured calls with a workspace of their own each, replayed in turn and on two streams"""
+    (m, n), ks = i8_shapes.TILES["T128Two"]
+    k = ks[-1]
+    assert lib.mm_i8_rows_scratch_bytes(True, m, n, k) > 0
+    q, s = lib.quantize_rows_i8(_rand(13, (m, k), torch.bfloat16).cuda())
+    sets = []
+    for i in range(2):
+        w = torch.randint(-1, 2, (n, k, 1, 1), generator=torch.Generator().manual_seed(40 + i)).float().cuda()
+        sets.append((lib.pack_weights(w, torch.full((n,), 0.5, device="cuda"), True), torch.full((n,), 0.5 + i, device="cuda")))
+    want = [lib.mm_i8_rows(q, s, rows, scale, n, k, True) for rows, scale in sets]
+    assert not torch.equal(want[0], want[1])
+    graphs, got = [], []
+    for rows, scale in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(lib.mm_i8_rows(q, s, rows, scale, n, k, True))
+        graphs.append(g)
+    sides = [torch.cuda.Stream() for _ in graphs]
+    for i in range(4):
+        for y in got:
+            y.zero_()
+        torch.cuda.synchronize()
+        for g, side in zip(graphs, sides):
+            with torch.cuda.stream(side if i % 2 else torch.cuda.current_stream()):
+                g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_more_rows_than_a_launch_holds():
+    rows = (1 << 23) + 3
+    x = torch.randn((rows, 16), dtype=torch.bfloat16, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    q, s = lib.quantize_rows_i8(x)
+    at = torch.tensor([0, 1, (1 << 23) - 1, 1 << 23, rows - 1], device="cuda")
+    _same_codes(x[at].cpu(), q[at], s[at])
+    most = x.float().abs().amax(1).cpu().double()
+    assert torch.equal(s.cpu(), (most / 127).float())   # (a quotient of 24 bits by 7 is no tie in 53)
+
+
 def test_refusals():
     q, s = (t.cuda() for t in _codes(1, 4, 64))
     w, ws = (t.cuda() for t in _codes(2, 8, 64))
