@@ -36,7 +36,7 @@ inline I8Form i8_form(int64_t M, int64_t N, int K) { return i8_estimate(M, N, K)
 // weights under up to 16 tokens or a chipful of the smallest workgroups, the form is the first of a list with about one workgroup per compute unit or
 // fewer: the smaller ones spread the work, the larger ones read less of the other operand again.  Codes, us: 1 x 4096 x 4096 (1,1) 6.1, (2,1) 6.6,
 // tiles 9.9; 1 x 8192 x 4096 10.5, 8.8, 9.9; 1 x 14336 x 4096 14.9, 12.7, 11.3; 32 x 4096 x 4096 (1,1) 10.3, (1,2) 8.3, tiles 9.9;
-// 64 x 1024 x 1024 (1,1) 3.7, tiles 5.2; 64 x 4096 x 4096 (2,2) 10.1, tiles 10.1.  Packed weights: 1 x 16384 x 16384 (1,1) 25.3, (4,1) 19.1.
+// 64 x 1024 x 1024 (1,1) 3.7, tiles 5.2; 64 x 4096 x 4096 (2,2) 10.1, tiles 10.1.  Packed weights: 16 x 16384 x 16384 (1,1) 40.5, (4,1) 23.5.
 //
 // More tokens over packed weights go by an estimate: microseconds of 128 codes of K for a round of 256 workgroups, and for tiles those above with the
 // launch that unpacks the weights (4 us and 0.18 for a million codes).  us, (4,1), (4,2), (4,4), tiles: 64 x 4096 x 4096 7.4, 8.7, 12.6, 24.4;

@@ -186,7 +186,7 @@ __device__ __forceinline__ void unpack32(uint32_t s, uint32_t z, uint32_t (&out)
 // Few tokens: KS wavefronts split K over one tile of 16 NB weight rows x 16 MB tokens and meet in LDS.  Operands come straight from memory
 // into registers, the next step's while this one is multiplied.  What a compute unit can have on its way through its L1 bounds codes (17 bytes per clock; two,
 // three or four steps ahead are no faster than one), 1 x 4096 x 4096 6.1 us with its launch; packed weights are bounded by memory for one token (16384 x 16384
-// ternary 17.6 us, 3.8 TB/s) and by unpacking, 4 instructions per word of codes, for many.
+// ternary 17.6 us, 3.8 TB/s, from HBM) and by unpacking, 4 instructions per word of codes, for many.
 template <I8Weights W, typename T, int NB, int MB, bool TOKENS>
 __global__ __launch_bounds__(512) void k_i8_few(I8Product p, uint32_t ntiles) {
     constexpr int KS = 8, LD = 16 * NB + 4;
@@ -266,11 +266,12 @@ __global__ __launch_bounds__(512) void k_i8_few(I8Product p, uint32_t ntiles) {
             }
             if constexpr (TOKENS) {
 #pragma unroll
-                for (int d = 0; d < 8; d++) x.t[d] = token_piece(0, q0 * 256 + 128 * (d / 2) + 32 * g + 16 * (d % 2));
+                for (int d = 0; d < 8; d++) x.t[d] = token_piece(0, q * 256 + half * 128 + 16 * d);
             }
         };
         // word d of quarter g <-> word g of quarter d: then the loads of a word's tokens take 128 codes side by side, whole cache lines, and not 32 each
-        // of four (us without / with: 128 x 4096 x 14336 by (4,2) 25.1 / 22.3, 256 x 4096 x 4096 by (4,4) 19.8 / 13.2)
+        // of four (us without / with: 128 x 4096 x 14336 by (4,2) 25.1 / 22.3, 256 x 4096 x 4096 by (4,4) 19.8 / 13.2).  Up to four tokens
+        // (TOKENS) have room in the L1 as they are: 1 x 16384 x 16384, weights in the last-level cache, 19.0 / 14.7 without
         auto turn = [&](v4u& w) {
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
@@ -285,10 +286,12 @@ __global__ __launch_bounds__(512) void k_i8_few(I8Product p, uint32_t ntiles) {
         };
         auto multiply = [&](int q0, Step& x) {
             const int k0 = q0 * 256 + 32 * g;
+            if constexpr (!TOKENS) {
 #pragma unroll
-            for (int j = 0; j < NB; j++) {
-                turn(x.s[j]);
-                if constexpr (TERN) turn(x.z[j]);
+                for (int j = 0; j < NB; j++) {
+                    turn(x.s[j]);
+                    if constexpr (TERN) turn(x.z[j]);
+                }
             }
 #pragma unroll
             for (int d = 0; d < 4; d++) {
@@ -415,7 +418,7 @@ static hipError_t launch_few(I8Few f, int dtype, const I8Product& p, hipStream_t
             kern<<<dim3((unsigned)tiles), dim3(512), bytes, st>>>(p, (uint32_t)ntiles);
             return hipGetLastError();
         };
-        // packed weights: a token's codes are asked for a step ahead up to four tokens; of more they fill the L1.  us, ahead / not: 1 x 16384 x 16384 18.0 / 21.7,
+        // packed weights: a token's codes are asked for a step ahead up to four tokens; of more they fill the L1.  us, ahead / not, before the turn above: 1 x 16384 x 16384 18.0 / 21.7,
         // 1 x 4096 x 14336 7.0 / 8.5, 16 x 16384 x 16384 26.6 / 23.9, 16 x 4096 x 4096 5.9 / 5.3
         auto run = [&](auto nb, auto mb) {
             if constexpr (W != I8Weights::Codes && decltype(mb)::value == 1)
