@@ -399,8 +399,10 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4 kv, T* K, T* V) {
 //     sum_t p_t v_td = sum_t w_t c_td - 8 sum_t w_t + sum_t p_t (vz_t + 8 vs_t),   w_t = p_t vs_t
 // with w_t rounded to float16 (where the result is float16: the sum of two) in both of its sums, so that its rounding only meets code - 8,
 // which is what is rounded where values are multiplied.  Queries are scaled by a power of two so that their largest
-// magnitude is in [2^14, 2^15): a float16 or bfloat16 keeps all of its bits, down to 2^-38 of the largest.  Weights are scaled by a power of
-// two that follows the largest vs so far, to at most 2^13 and 2^5 where the largest score so far is their measure: what is below 2^-25 of that is lost.
+// magnitude is in [2^14, 2^15): a float16 or bfloat16 keeps all of its bits, down to 2^-38 of the largest.  Weights have a unit of their own in
+// each row, a power of two that follows the largest p vs that the row has met (not the largest vs: a token that the row does not see, or hardly, does not move it): that
+// one is 2^6 or more, at most 2^15, and what is below 2^-27 of it is lost.  What weights are relative to is a power of two as well, so
+// that both move without a rounding.
 //
 // A step is 32 tokens of one wavefront.  Keys are the A operand: row r of block b (two blocks of 16) is token 8 (r / 4) + 4 b + r % 4, so that
 // lane quarter g ends with the scores of tokens 8 g .. 8 g + 7 of its column (a query), in the order in which the second product takes
@@ -621,15 +623,17 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT, D * CB <= 256 && D < 256 ?
         unit[b] = fminf(fmaxf(__builtin_ldexpf(p.scale2, 24 - up), 0x1p-126f), 0x1.fffffep127f);
     }
     v4f o[CB][NB], wsum[CB];
-    float m[CB], limit[CB], l[CB], zsum[CB];   // m: what the weights are relative to, a power of two
+    float m[CB], limit[CB], l[CB], zsum[CB];   // m: what the weights are relative to, a whole power of two
+    float one[CB];                             // what a weight of 1 (times kScales) is in float16, a power of two: the rows' units
 #pragma unroll
     for (int b = 0; b < CB; b++) {
 #pragma unroll
         for (int i = 0; i < NB; i++) o[b][i] = v4f{0, 0, 0, 0};
-        wsum[b] = v4f{0, 0, 0, 0}, m[b] = limit[b] = -__builtin_inff(), l[b] = zsum[b] = 0.0f;
+        wsum[b] = v4f{0, 0, 0, 0}, m[b] = limit[b] = -__builtin_inff(), l[b] = zsum[b] = 0.0f, one[b] = power(254);
     }
     const v4u eights = {0x00080008u, 0x00800080u, 0x00080008u, 0x00800080u};   // 8 in units of the codes
-    int vexp = 6;   // biased exponent of the largest vs so far: weights are scaled by 2^(131 - vexp)
+    constexpr float kScales = 0x1p-12f;   // times the largest scale a weight of 2^8 is a float
+    auto exponent = [](float x) { return (int)(__builtin_bit_cast(uint32_t, x) >> 23); };   // biased, of x >= 0
 
     // EDGE: some row does not see all of the step's tokens
     // keys_done, values_done: called when those of the step are not needed any more
@@ -640,20 +644,11 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT, D * CB <= 256 && D < 256 ?
 #pragma unroll
             for (int e = 0; e < 8; e++) x.vp[e] = x.there && t0 + 8 * g + e < held ? x.vp[e] : 0u;   // behind the sequence: not looked at
         }
-        float largest = 0.0f;   // (NaN, the scale of a token of NaN, is passed over)
-#pragma unroll
-        for (int e = 0; e < 8; e++) largest = fmaxf(largest, scale_of(x.vp[e]));
-        largest = max_over_quarters(largest);
-        const int grown = __builtin_amdgcn_readfirstlane(max(vexp, min((int)(__builtin_bit_cast(uint32_t, largest) >> 23), 254)));   // (columns share their tokens)
-        const float shrink = grown != vexp ? power(max(127 - (grown - vexp), 0)) : 1.0f;
-        const bool new_scale = grown != vexp;
-        vexp = grown;
-        const float even = power(258 - vexp), odd = even * 0.0625f;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float sc = scale_of(x.vp[e]);
             vz[e] = __builtin_fmaf(8.0f, sc, zero_of(x.vp[e]));
-            vs[e] = sc * ((e & 1) ? odd : even);
+            vs[e] = sc * ((e & 1) ? kScales / 16 : kScales);
         }
         float sc[CB][8];
         {
@@ -693,20 +688,23 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT, D * CB <= 256 && D < 256 ?
             float top = sc[cb][0];
 #pragma unroll
             for (int e = 1; e < 8; e++) top = fmaxf(top, sc[cb][e]);
-            top = max_over_quarters(top);
             // what the weights are relative to moves when it is passed by more than 2^8 (and by the first tokens that a row sees): they and their sums
             // have room for that, and most steps need not touch the sums (500 -> 364 us, with the steps that look at each token in a loop of their own)
-            if (new_scale || __any(top * unit[cb] > limit[cb])) {
-                const bool move = top * unit[cb] > limit[cb];
-                const float to = move ? top * unit[cb] : m[cb], f = move ? __builtin_amdgcn_exp2f(m[cb] - to) : 1.0f, fo = f * shrink;
+            if (__any(top * unit[cb] > limit[cb])) {
+                const float reach = max_over_quarters(top) * unit[cb];
+                const bool move = reach > limit[cb];
+                const float to = move ? __builtin_ceilf(reach) : m[cb];
+                const int by = move ? (int)fminf(to - m[cb], 512.0f) : 0;   // the row's unit goes up with it, as far as it may
+                const int held = exponent(one[cb]), next = min(held + by, 254);
+                const float f = __builtin_ldexpf(1.0f, -by), fo = __builtin_ldexpf(1.0f, next - held - by);
                 l[cb] *= f, zsum[cb] *= f, wsum[cb] *= fo;
 #pragma unroll
                 for (int i = 0; i < NB; i++) o[cb][i] *= fo;
-                m[cb] = to, limit[cb] = to + 8.0f;
+                m[cb] = to, limit[cb] = to + 8.0f, one[cb] = power(next);
             }
             const float off = m[cb] == -__builtin_inff() ? 0.0f : -m[cb];
             uint32_t hi[4], lo[4];
-            float w[8];
+            float w[8], most = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[cb][e], unit[cb], off));
@@ -714,7 +712,19 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT, D * CB <= 256 && D < 256 ?
                 const bool hidden = EDGE && (!x.there || t0 + 8 * g + e >= seen[cb]);   // what a row does not see may be no number
                 zsum[cb] = hidden ? zsum[cb] : __builtin_fmaf(y, vz[e], zsum[cb]);
                 w[e] = hidden ? 0.0f : y * vs[e];
+                most = fmaxf(most, __builtin_fabsf(w[e]));   // (NaN, of a token of NaN, is passed over)
             }
+            if (__any(most * one[cb] > 0x1p15f)) {   // the row's unit goes down
+                most = max_over_quarters(most);
+                const int held = exponent(one[cb]), next = most * one[cb] > 0x1p15f ? 260 - min(exponent(most), 254) : held;
+                const float fo = __builtin_ldexpf(1.0f, next - held);
+                wsum[cb] *= fo;
+#pragma unroll
+                for (int i = 0; i < NB; i++) o[cb][i] *= fo;
+                one[cb] = power(next);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] *= one[cb];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 hi[e] = pack_f16(w[e], w[e + 4]);
@@ -768,10 +778,10 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT, D * CB <= 256 && D < 256 ?
             }
     }
     // channel (4 g + e) NB + i of a row is in accumulator e of block i
-    const float back = power(vexp - 4);   // 1 / the weights' scale, and 2^24 for the codes
     auto row_at = [&](uint32_t r) { return (int64_t)(first + (int)(r / group)) * p.heads_q + head * p.group + (int)(r % group); };
 #pragma unroll
     for (int b = 0; b < CB; b++) {
+        const int back = 163 - exponent(one[b]);   // of the row's unit, kScales and the codes: 2^(127 + 12 + 24 - exponent)
         l[b] = sum_over_quarters(l[b]), zsum[b] = sum_over_quarters(zsum[b]);
         if constexpr (WT == 1) {
             const uint32_t r = row0 + 16 * b + c;
@@ -782,7 +792,7 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT, D * CB <= 256 && D < 256 ?
             for (int e = 0; e < 4; e++) {
                 T v[NB];
 #pragma unroll
-                for (int i = 0; i < NB; i++) v[i] = (T)(l[b] == 0.0f ? 0.0f : __builtin_fmaf((o[b][i][e] - wsum[b][e]) * 0x1p24f, back, zsum[b]) * f);
+                for (int i = 0; i < NB; i++) v[i] = (T)(l[b] == 0.0f ? 0.0f : (__builtin_ldexpf(o[b][i][e] - wsum[b][e], back) + zsum[b]) * f);
                 __builtin_memcpy(static_cast<T*>(p.out) + at * D + (4 * g + e) * NB, v, sizeof(v));
             }
         } else {   // the wavefronts meet
@@ -791,7 +801,7 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT, D * CB <= 256 && D < 256 ?
 #pragma unroll
             for (int i = 0; i < NB; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) mine[(4 * g + e) * NB + i] = __builtin_fmaf((o[b][i][e] - wsum[b][e]) * 0x1p24f, back, zsum[b]);
+                for (int e = 0; e < 4; e++) mine[(4 * g + e) * NB + i] = __builtin_ldexpf(o[b][i][e] - wsum[b][e], back) + zsum[b];
             float* const ml = lds + WT * TILE * LD;
             if (g == 0) ml[(wave * TILE + 16 * b + c) * 2] = m[b], ml[(wave * TILE + 16 * b + c) * 2 + 1] = l[b];
         }

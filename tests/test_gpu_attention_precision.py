@@ -1,0 +1,65 @@
+"""Attention over the 4-bit cache held to the bound of its arithmetic (tests/attention_bound.py), where that can go wrong."""
+import pytest
+
+torch = pytest.importorskip("torch")
+import fastertnn_amd.lib as lib
+from tests import attention_bound, attention_cases as cases
+
+pytestmark = pytest.mark.gpu
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _run(call, max_len=0):
+    cache, table, lens, starts, q = call
+    return lib.kv4_attention(q.cuda(), cache.raw().cuda(), table.cuda(), lens.cuda(), starts.cuda(), cache.heads, cache.page, max_len=max_len).cpu()
+
+
+def _check(call, max_len=0):
+    out = _run(call, max_len)
+    want, slack = attention_bound.bound(*call)
+    off = (out.double() - want).abs()
+    assert torch.isfinite(out).all()
+    assert bool((off <= slack).all()), "off by up to %.3g of the allowed" % float((off / slack).max())
+    return out
+
+
+def _many(heads, group, dim, new):
+    """rows enough that wavefronts have all tokens of theirs"""
+    assert new * group // (64 if dim == 256 else 128) * heads >= 480
+    return heads, group, dim
+
+
+# heads, group, dim, page, tokens, new ones
+FORMS = [(1, 4, 64, 16, 300, 5), (2, 4, 128, 64, 300, 1), (1, 3, 96, 32, 90, 40), (1, 2, 256, 16, 200, 9), (16, 4, 64, 32, 1100, 1000), (12, 5, 128, 64, 1100, 1050), (16, 2, 256, 128, 1100, 1000)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,group,dim,page,length,new", FORMS)
+def test_a_token_of_large_values_that_rows_do_not_see(heads, group, dim, page, length, new, dtype):
+    """the rows before it have the bits that they have without it"""
+    if new >= 1000:
+        _many(heads, group, dim, new)
+    call = cases.unseen(heads, group, dim, page, length, max(new, 2), 2.0 ** 20, TYPES[dtype])
+    out = _check(call)
+    assert torch.equal(out[:-1], _run(cases.unseen(heads, group, dim, page, length, max(new, 2), 1.0, TYPES[dtype]))[:-1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ratio", [2.0 ** 12, 2.0 ** 20, 2.0 ** 40])
+@pytest.mark.parametrize("heads,group,dim,page,length,new", FORMS)
+def test_tokens_of_large_values_and_no_weight(heads, group, dim, page, length, new, ratio, dtype):
+    """the first token of the sequence, one in the middle and one that the last step holds"""
+    call = cases.weightless(heads, group, dim, page, [length], [1 if new < 1000 else new], ratio, TYPES[dtype], (0, length // 2, length - 2) if new < 1000 else (0, 40, 45))
+    _check(call)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,group,dim,page,length,new", FORMS)
+def test_tokens_of_all_scales(heads, group, dim, page, length, new, dtype):
+    _check(cases.mixed(heads, group, dim, page, [length], [new], 6, TYPES[dtype]))
+
+
+@pytest.mark.parametrize("max_len", [0, 4000])
+def test_tokens_of_large_values_over_parts(max_len):
+    """split over workgroups and wavefronts, most of which hold none of them"""
+    _check(cases.weightless(1, 4, 128, 64, [4000], [1], 2.0 ** 30, torch.bfloat16, (0, 1333, 2666, 3998)), max_len)
