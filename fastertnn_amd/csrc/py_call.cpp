@@ -15,7 +15,6 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <algorithm>
 #include <climits>
 
 #include "../../include/ftnn.h"
@@ -197,7 +196,8 @@ struct Tensors {
         return s == at::kFloat ? FTNN_F32 : s == at::kHalf ? FTNN_F16 : FTNN_BF16;
     }
 };
-int64_t row_stride(const at::Tensor& t, int64_t least) { return t.size(0) > 1 ? t.stride(0) : std::max(least, t.size(1)); }
+// values between rows of `least` or more; whatever torch says of a single row, and however wide that is
+int64_t row_stride(const at::Tensor& t, int64_t least) { return t.size(0) > 1 ? t.stride(0) : least; }
 
 // what fn() answers: the library's status where it refused, nothing where a tensor was not plain after all
 template <typename F>

@@ -407,8 +407,8 @@ def _flat(t, name, dtype, shape):
 
 
 def _row_stride(t, least):
-    """values between rows; whatever torch says of a single row"""
-    return t.stride(0) if t.shape[0] > 1 else max(least, t.shape[1])
+    """values between rows of `least` or more; whatever torch says of a single row, and however wide that is"""
+    return t.stride(0) if t.shape[0] > 1 else least
 
 
 def i8_row_bytes(k):
