@@ -209,14 +209,16 @@ PyObject* answer(F&& fn) {
         Py_RETURN_NONE;
     }
 }
+// fn(stream) with the lock of the interpreter released.  What fn takes is plain values: a tensor's data are asked for before, since that may throw (a tensor
+// without storage has the sizes of any other)
 template <typename F>
 int unlocked(F&& fn) {
-    int rc;
     void* const stream = c10::hip::getCurrentHIPStream().stream();
-    Py_BEGIN_ALLOW_THREADS
-    rc = fn(stream);
-    Py_END_ALLOW_THREADS
-    return rc;
+    struct Released {
+        PyThreadState* const state = PyEval_SaveThread();
+        ~Released() { PyEval_RestoreThread(state); }
+    } released;
+    return fn(stream);
 }
 
 // x, q, scale
@@ -230,9 +232,8 @@ PyObject* quantize_rows_i8(PyObject*, PyObject* const* v, Py_ssize_t n) {
         if (!r.good) Py_RETURN_NONE;
         const int64_t rows = x.size(0), k = x.size(1), nb = ftnn_i8_row_bytes((int)k);
         const at::Tensor q = at::empty({rows, nb}, x.options().dtype(at::kChar)), s = at::empty({rows}, x.options().dtype(at::kFloat));
-        const int rc = unlocked([&](void* st) {
-            return ftnn_quantize_rows_i8(dtype, x.data_ptr(), row_stride(x, k), rows, (int)k, static_cast<int8_t*>(q.data_ptr()), nb, static_cast<float*>(s.data_ptr()), st);
-        });
+        const int rc = unlocked([dtype, xp = x.data_ptr(), x_stride = row_stride(x, k), rows, k, qp = static_cast<int8_t*>(q.data_ptr()), nb,
+                                 sp = static_cast<float*>(s.data_ptr())](void* st) { return ftnn_quantize_rows_i8(dtype, xp, x_stride, rows, (int)k, qp, nb, sp, st); });
         if (rc) return PyLong_FromLong(rc);
         return Py_BuildValue("NN", THPVariable_Wrap(q), THPVariable_Wrap(s));
     });
@@ -275,13 +276,13 @@ PyObject* product(PyObject* const* v, bool packed) {
             scratch = at::empty({have = need}, a.options().dtype(at::kByte));
         }
         if (!out.defined()) out = at::empty({m, n}, a.options().dtype(type));
-        const int64_t out_stride = row_stride(out, n);
-        const int rc = unlocked([&](void* st) {
-            const int8_t* const codes = static_cast<const int8_t*>(a.data_ptr());
-            if (packed)
-                return ftnn_mm_i8_rows(ternary, dtype, codes, row_stride(a, nb), sa, static_cast<const int64_t*>(b.data_ptr()), sb, bias, m, n, (int)k, out.data_ptr(), out_stride,
-                                       scratch.defined() ? scratch.data_ptr() : nullptr, have, st);
-            return ftnn_mm_i8(dtype, codes, row_stride(a, nb), sa, static_cast<const int8_t*>(b.data_ptr()), row_stride(b, nb), sb, bias, m, n, (int)k, out.data_ptr(), out_stride, st);
+        const int8_t* const codes = static_cast<const int8_t*>(a.data_ptr());
+        const void* const weights = b.data_ptr();
+        void *const y = out.data_ptr(), *const work = scratch.defined() ? scratch.data_ptr() : nullptr;
+        const int64_t a_stride = row_stride(a, nb), b_stride = packed ? 0 : row_stride(b, nb), out_stride = row_stride(out, n);
+        const int rc = unlocked([=](void* st) {
+            if (packed) return ftnn_mm_i8_rows(ternary, dtype, codes, a_stride, sa, static_cast<const int64_t*>(weights), sb, bias, m, n, (int)k, y, out_stride, work, have, st);
+            return ftnn_mm_i8(dtype, codes, a_stride, sa, static_cast<const int8_t*>(weights), b_stride, sb, bias, m, n, (int)k, y, out_stride, st);
         });
         return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
     });
@@ -334,10 +335,14 @@ PyObject* kv4_append(PyObject*, PyObject* const* v, Py_ssize_t n) {
         const int neighbours = r.truth(v[10]);
         if (!r.good) Py_RETURN_NONE;
         if (q.defined()) q_out = at::empty(q.sizes(), q.options());
-        const int rc = unlocked([&](void* st) {
-            const bool with = q.defined();
-            return ftnn_kv4_append(&kv, dtype, k.data_ptr(), k.stride(0), k.stride(1), val.data_ptr(), val.stride(0), val.stride(1), cos, sin, positions, rot, neighbours,
-                                   with ? (int)q.size(1) : 0, with ? q.data_ptr() : nullptr, with ? q.stride(0) : 0, with ? q.stride(1) : 0, with ? q_out.data_ptr() : nullptr, st);
+        struct Rows {
+            void* p = nullptr;
+            int64_t token = 0, head = 0;
+            int heads = 0;
+        };
+        auto rows = [](const at::Tensor& t) { return t.defined() ? Rows{t.data_ptr(), t.stride(0), t.stride(1), (int)t.size(1)} : Rows{}; };
+        const int rc = unlocked([=, &kv, kr = rows(k), vr = rows(val), qr = rows(q), to = rows(q_out).p](void* st) {
+            return ftnn_kv4_append(&kv, dtype, kr.p, kr.token, kr.head, vr.p, vr.token, vr.head, cos, sin, positions, rot, neighbours, qr.heads, qr.p, qr.token, qr.head, to, st);
         });
         if (rc) return PyLong_FromLong(rc);
         return Py_BuildValue("(N)", q.defined() ? THPVariable_Wrap(q_out) : Py_NewRef(Py_None));
@@ -356,7 +361,7 @@ PyObject* kv4_read(PyObject*, PyObject* const* v, Py_ssize_t n) {
         if (!r.need(tokens >= 0) || !cache_of(r, v, tokens, heads, dim, r.integer(v[7]), &kv)) Py_RETURN_NONE;
         const auto options = THPVariable_Unpack(v[0]).options().dtype(type);
         const at::Tensor k = at::empty({tokens, heads, dim}, options), val = at::empty({tokens, heads, dim}, options);
-        const int rc = unlocked([&](void* st) { return ftnn_kv4_read(&kv, dtype, k.data_ptr(), val.data_ptr(), st); });
+        const int rc = unlocked([&kv, dtype, kp = k.data_ptr(), vp = val.data_ptr()](void* st) { return ftnn_kv4_read(&kv, dtype, kp, vp, st); });
         if (rc) return PyLong_FromLong(rc);
         return Py_BuildValue("NN", THPVariable_Wrap(k), THPVariable_Wrap(val));
     });
@@ -390,9 +395,8 @@ PyObject* kv4_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
             scratch = at::empty({have}, q.options().dtype(at::kByte));
         }
         const float scale = (float)PyFloat_AS_DOUBLE(v[7]);
-        const int rc = unlocked([&](void* st) {
-            return ftnn_kv4_attention(&kv, dtype, heads_q, q.data_ptr(), q.stride(0), q.stride(1), scale, (int)max_len, out.data_ptr(), scratch.defined() ? scratch.data_ptr() : nullptr,
-                                      have, st);
+        const int rc = unlocked([=, &kv, qp = q.data_ptr(), token = q.stride(0), head = q.stride(1), y = out.data_ptr(), work = scratch.defined() ? scratch.data_ptr() : nullptr](void* st) {
+            return ftnn_kv4_attention(&kv, dtype, heads_q, qp, token, head, scale, (int)max_len, y, work, have, st);
         });
         return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
     });
