@@ -398,7 +398,9 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4 kv, T* K, T* V) {
 //     q . k_t = ks_t sum_d q_d c_td + kz_t sum_d q_d
 //     sum_t p_t v_td = sum_t w_t c_td - 8 sum_t w_t + sum_t p_t (vz_t + 8 vs_t),   w_t = p_t vs_t
 // with w_t rounded to float16 (where the result is float16: the sum of two) in both of its sums, so that its rounding only meets code - 8,
-// which is what is rounded where values are multiplied.  Queries are scaled by a power of two so that their largest
+// which is what is rounded where values are multiplied.  The two sums on w grow with the length while their difference does not: every 16 steps the second is taken off the
+// first, so that they hold 512 tokens at most (131072 tokens without it: off by 3e-5 of the weights, so 1e-7, for 2 % of a prompt's time; -8 as one more operand of each
+// block of channels, so that no sum grows at all, costs 12 to 19 %).  Queries are scaled by a power of two so that their largest
 // magnitude is in [2^14, 2^15): a float16 or bfloat16 keeps all of its bits, down to 2^-38 of the largest.  Weights have a unit of their own in
 // each row, a power of two that follows the largest p vs that the row has met (not the largest vs: a token that the row does not see, or hardly, does not move it): that
 // one is 2^6 or more, at most 2^15, and what is below 2^-27 of it is lost.  What weights are relative to is a power of two as well, so
@@ -737,6 +739,14 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT, D * CB <= 256 && D < 256 ?
             if (PARTS == 2) wl[PARTS == 2 ? cb : 0] = __builtin_bit_cast(v8h, (v4u{lo[0], lo[1], lo[2], lo[3]}));
         }
         __builtin_amdgcn_sched_barrier(0);
+        if ((t0 / (32 * WT)) % 16 == 0) {   // 8 times the weights so far, off the sums of codes
+#pragma unroll
+            for (int cb = 0; cb < CB; cb++) {
+#pragma unroll
+                for (int i = 0; i < NB; i++) o[cb][i] -= wsum[cb];
+                wsum[cb] = v4f{0, 0, 0, 0};
+            }
+        }
 #pragma unroll
         for (int i = 0; i <= NB; i++) {
             const v8h a = i == NB ? __builtin_bit_cast(v8h, eights) : codes8(x.vw[i == NB ? 0 : i]);

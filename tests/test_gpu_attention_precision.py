@@ -63,3 +63,13 @@ def test_tokens_of_all_scales(heads, group, dim, page, length, new, dtype):
 def test_tokens_of_large_values_over_parts(max_len):
     """split over workgroups and wavefronts, most of which hold none of them"""
     _check(cases.weightless(1, 4, 128, 64, [4000], [1], 2.0 ** 30, torch.bfloat16, (0, 1333, 2666, 3998)), max_len)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sums_do_not_grow_with_the_length(dtype):
+    """131072 tokens in one wavefront's sums, whose values cancel step by step.  In 16 steps sums of code * weight and of 8 * weight grow to 9 and 8 times the weights of
+    those steps, half of that in the mean, and each step rounds both, by up to 2 u of them where what does not fit is cut off: 16 * 17 u = 272 u of the weights, and
+    no more over all steps together.  (Sums over all tokens are as large as 9 times all weights, in each of 4096 steps.)"""
+    call = cases.cancelling(2, 16383, 64, 131072, 2, TYPES[dtype])
+    out = _run(call).double()
+    assert float(out.square().mean().sqrt()) <= 272 * 2.0 ** -24 * 1024
