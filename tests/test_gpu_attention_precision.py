@@ -73,3 +73,19 @@ def test_sums_do_not_grow_with_the_length(dtype):
     call = cases.cancelling(2, 16383, 64, 131072, 2, TYPES[dtype])
     out = _run(call).double()
     assert float(out.square().mean().sqrt()) <= 272 * 2.0 ** -24 * 1024
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,group,dim,lens,new", [(2, 4, 128, [5, 16, 33, 48, 330, 650], [1] * 6), (1, 8, 64, [1290, 17], [1, 1]), (1, 4, 256, [1001, 500], [3, 2]), (12, 5, 128, [1290], [1050]), (16, 4, 64, [1101], [1000])])
+def test_what_the_table_holds_behind_the_sequences(heads, group, dim, lens, new, dtype):
+    """pages of 16 tokens, half of a step: good pages behind the last one, bad ones, none at all"""
+    cache, table, ln, starts, g = cases.make(heads, dim, 16, [max(lens) + 64] * len(lens), new, 6)
+    ln = torch.tensor(lens, dtype=torch.int32)
+    q = torch.randn((int(starts[-1]), heads * group, dim), generator=g).to(TYPES[dtype])
+    want, slack = attention_bound.bound(cache, table, ln, starts, q)
+    good = _run((cache, table, ln, starts, q), max(lens))
+    assert bool(((good.double() - want).abs() <= slack).all())
+    behind = torch.arange(table.shape[1]) >= (ln[:, None] + 15) // 16
+    for bad in (-1, 1 << 30):
+        assert torch.equal(_run((cache, torch.where(behind, bad, table), ln, starts, q), max(lens)), good)
+    assert torch.equal(_run((cache, table[:, :(max(lens) + 15) // 16].contiguous(), ln, starts, q), max(lens)), good)
