@@ -89,3 +89,25 @@ def test_what_the_table_holds_behind_the_sequences(heads, group, dim, lens, new,
     for bad in (-1, 1 << 30):
         assert torch.equal(_run((cache, torch.where(behind, bad, table), ln, starts, q), max(lens)), good)
     assert torch.equal(_run((cache, table[:, :(max(lens) + 15) // 16].contiguous(), ln, starts, q), max(lens)), good)
+
+
+# from one token to thousands, ragged, odd numbers of heads: tokens split over wavefronts and workgroups, and wavefronts on all tokens
+SHAPES = [(1, 1, 64, 16, [1], [1]), (2, 4, 128, 64, [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200, 257], [1] * 16), (1, 8, 96, 32, [100, 31], [1, 1]),
+          (2, 2, 256, 16, [77, 300], [1, 1]), (1, 20, 64, 32, [90, 40], [1, 1]), (2, 3, 64, 16, [40, 9, 100], [40, 1, 33]), (4, 4, 128, 32, [70, 64, 31], [5, 64, 1]),
+          (2, 5, 256, 256, [280], [23]), (2, 4, 128, 64, [3000, 40, 1], [1, 1, 1]), (1, 6, 64, 16, [2500], [3]), (32, 2, 64, 64, [700, 300, 200], [600, 300, 123]),
+          (16, 4, 128, 16, [990, 64, 1], [900, 64, 1]), (16, 5, 96, 32, [500, 420], [400, 419]), (8, 4, 256, 16, [1000, 70], [930, 70])]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,group,dim,page,lens,new", SHAPES)
+def test_within_the_bound_of_its_arithmetic(heads, group, dim, page, lens, new, dtype):
+    cache, table, ln, starts, g = cases.make(heads, dim, page, lens, new, dim + page + len(lens))
+    q = torch.randn((int(starts[-1]), heads * group, dim), generator=g).to(TYPES[dtype])
+    _check((cache, table, ln, starts, q))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,group,dim,page,sequences", [(2, 64, 64, 16, 1), (1, 30, 128, 32, 3), (1, 17, 96, 16, 2), (1, 16, 256, 64, 1), (8, 512, 64, 32, 16)])
+def test_the_rounding_of_the_weights(heads, group, dim, page, sequences, dtype):
+    """what a float16 result is held to takes both parts of its weights (one: 14 times the bound), what a bfloat16 result is held to takes float16 and not bfloat16"""
+    _check(cases.two_halves(heads, group, dim, page, TYPES[dtype], sequences))
