@@ -951,12 +951,15 @@ Kv4Plan plan_of(const ftnn_kv4_t& kv, int heads_q, int max_len) {
     return {1, 4, narrow, splits};
 }
 
+constexpr int kMostWorkgroups = 1 << 24;   // of 256 threads along a side: a launch holds fewer than 2^32
+
 }  // namespace
 
 hipError_t launch_kv4_append(const ftnn_kv4_t& kv, int dtype, const Kv4Rows& k, const Kv4Rows& v, const Kv4Rotation& r, int heads_q,
                              const Kv4Rows& q, void* d_q_out, hipStream_t st) {
     const Kv4 dv = device_view(kv);
     const int eights = eights_of(kv), groups = (kv.heads + heads_q + 3) / 4;
+    if (eights >= kMostWorkgroups) return hipErrorInvalidConfiguration;
     const int heads_at_a_time = std::max(1, std::min(groups, (512 + eights - 1) / eights));   // about two workgroups per compute unit, or all there are
     return with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
@@ -969,6 +972,7 @@ hipError_t launch_kv4_append(const ftnn_kv4_t& kv, int dtype, const Kv4Rows& k, 
 
 hipError_t launch_kv4_read(const ftnn_kv4_t& kv, int dtype, void* d_k, void* d_v, hipStream_t st) {
     const Kv4 dv = device_view(kv);
+    if (eights_of(kv) >= kMostWorkgroups) return hipErrorInvalidConfiguration;
     return with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
         return with_dim(kv.dim, [&](auto d) {
@@ -986,6 +990,7 @@ int64_t kv4_attention_scratch(const ftnn_kv4_t& kv, int heads_q, int max_len) {
 hipError_t launch_kv4_attention(const ftnn_kv4_t& kv, int dtype, int heads_q, const Kv4Rows& q, float scale, int max_len, void* d_out,
                                 void* d_scratch, hipStream_t st) {
     const Kv4Plan plan = plan_of(kv, heads_q, max_len);
+    if (plan.tiles >= kMostWorkgroups) return hipErrorInvalidConfiguration;
     Kv4Attend p;
     p.kv = device_view(kv), p.q = q, p.heads_q = heads_q, p.group = heads_q / kv.heads, p.splits = plan.splits;
     p.scale2 = scale * 1.44269504088896341f, p.out = d_out, p.part = static_cast<float*>(d_scratch);

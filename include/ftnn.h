@@ -417,6 +417,8 @@ FTNN_API int ftnn_mm_i8_rows(int ternary, int dtype, const int8_t *d_a, int64_t 
  * tensors, each with `tokens` rows.  starts[0] is 0 and starts do not fall.  Rows from starts[sequences] on are left as they are.
  * The arrays are read on the device: no call waits for it.  A page number outside of the cache is no error: its tokens
  * are not stored, read as zero and are not seen by attention.
+ * A call has fewer than 2^27 - 16 * sequences tokens, and for attention fewer than 2^24 tiles, of 16 to 128 rows (query heads of the tokens of one
+ * sequence over one head of keys) each: FTNN_EHIP beyond.
  */
 typedef struct ftnn_kv4 {
     void *d_cache;          /* 16-byte aligned                              */
