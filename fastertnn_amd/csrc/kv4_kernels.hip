@@ -169,8 +169,9 @@ __device__ __forceinline__ void rotate(const Kv4Rotation& r, int d, const Kv4Ang
 
 // scale and zero of a group whose smallest and largest values are given, as the cache holds them: two bfloat16 in a word
 __device__ __forceinline__ uint32_t make_params(float low, float high, float* scale, float* zero) {
-    // (times 1/15 in 64 bits: one rounding to fp32 is the quotient's)
-    const __bf16 z = (__bf16)low, s = (__bf16)(float)(((double)high - (double)low) * (1.0 / 15.0));
+    float fifteenth = (float)(((double)high - (double)low) * (1.0 / 15.0));   // (times 1/15 in 64 bits: one rounding to fp32 is the quotient's)
+    asm volatile("" : "+v"(fifteenth));   // in fp32 from here on: the compiler would make one rounding of this and the next
+    const __bf16 z = (__bf16)low, s = (__bf16)fifteenth;
     *scale = (float)s, *zero = (float)z;
     if (!(__builtin_fabsf(*zero) < __builtin_inff())) {   // of a group with a NaN or an infinity, or a zero beyond bfloat16
         *scale = *zero = __builtin_nanf("");

@@ -439,8 +439,8 @@ FTNN_API int64_t ftnn_kv4_page_bytes(int heads, int dim, int page);
  * d_cos, d_sin[position][i], i < rot / 2, the pair (x1, x2) becomes (x1 cos - x2 sin, x2 cos + x1 sin), computed in 64 bits and rounded to
  * fp32; pairs are elements (i, i + rot / 2), or (2 i, 2 i + 1) if `neighbours` is set; elements from rot on stay (rot even, 0: no rotation,
  * d_cos and d_sin unused).  Then per token and head: zero = the smallest value and scale = (largest - smallest) / 15, both
- * rounded to bfloat16; code = (x - zero) / scale rounded to the nearest integer, ties to even, kept within 0 .. 15 (0 where scale is 0).
- * A group with a NaN, an infinity or a spread beyond fp32 gets scale and zero NaN.  With heads_q > 0 the queries d_q
+ * rounded to fp32 and that to bfloat16; code = (x - zero) / scale rounded to the nearest integer, ties to even, kept within 0 .. 15 (0 where scale is 0).
+ * A group with a NaN, an infinity or a smallest value beyond bfloat16 gets scale and zero NaN.  With heads_q > 0 the queries d_q
  * [tokens][heads_q][dim] of the same tokens are rotated into d_q_out, contiguous, in the same launch.  Strides in values; channels are
  * contiguous.  Tokens whose position is negative or not below `positions` (rows of the tables; not looked at if rot is 0) are not stored, and
  * their queries not written.  A page that receives tokens in a call belongs to one sequence.
