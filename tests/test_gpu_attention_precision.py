@@ -111,3 +111,11 @@ def test_within_the_bound_of_its_arithmetic(heads, group, dim, page, lens, new, 
 def test_the_rounding_of_the_weights(heads, group, dim, page, sequences, dtype):
     """what a float16 result is held to takes both parts of its weights (one: 14 times the bound), what a bfloat16 result is held to takes float16 and not bfloat16"""
     _check(cases.two_halves(heads, group, dim, page, TYPES[dtype], sequences))
+
+
+@pytest.mark.parametrize("exponent", [-100, 110])
+@pytest.mark.parametrize("heads,group,dim,page,length,new", FORMS)
+def test_values_at_the_ends_of_bfloat16(heads, group, dim, page, length, new, exponent):
+    call = cases.mixed(heads, group, dim, page, [length], [new], 6, torch.bfloat16)
+    call[0].vp *= 2.0 ** exponent
+    _check(call)
