@@ -399,8 +399,9 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4 kv, T* K, T* V) {
 //     q . k_t = ks_t sum_d q_d c_td + kz_t sum_d q_d
 //     sum_t p_t v_td = sum_t w_t c_td - 8 sum_t w_t + sum_t p_t (vz_t + 8 vs_t),   w_t = p_t vs_t
 // with w_t rounded to float16 (where the result is float16: the sum of two) in both of its sums, so that its rounding only meets code - 8,
-// which is what is rounded where values are multiplied.  The two sums on w grow with the length while their difference does not: every 16 steps the second is taken off the
-// first, so that they hold 512 tokens at most (131072 tokens without it: off by 3e-5 of the weights, so 1e-7, for 2 % of a prompt's time; -8 as one more operand of each
+// which is what is rounded where values are multiplied.  The three sums grow with the length while what they make together does not: every 16 steps the second and
+// third are joined to the first, which so holds outputs, and no other sum goes over more than 512 tokens (131072 tokens whose values cancel, about code 8 / about code 1:
+// off by 3e-5 / 5e-4 of the weights with each sum by itself, now 1e-7 / 2e-6, for 4 % of a prompt's time; -8 as one more operand of each
 // block of channels, so that no sum grows at all, costs 12 to 19 %).  Queries are scaled by a power of two so that their largest
 // magnitude is in [2^14, 2^15): a float16 or bfloat16 keeps all of its bits, down to 2^-38 of the largest.  Weights have a unit of their own in
 // each row, a power of two that follows the largest p vs that the row has met (not the largest vs: a token that the row does not see, or hardly, does not move it): that
@@ -740,12 +741,23 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT, D * CB <= 256 && D < 256 ?
             if (PARTS == 2) wl[PARTS == 2 ? cb : 0] = __builtin_bit_cast(v8h, (v4u{lo[0], lo[1], lo[2], lo[3]}));
         }
         __builtin_amdgcn_sched_barrier(0);
-        if ((t0 / (32 * WT)) % 16 == 0) {   // 8 times the weights so far, off the sums of codes
+        if ((t0 / (32 * WT)) % 16 == 0) {
 #pragma unroll
             for (int cb = 0; cb < CB; cb++) {
+                const float z = sum_over_quarters(zsum[cb]);
+                int held = exponent(one[cb]);
+                if (__any(exponent(__builtin_fabsf(z)) + held > 390)) {   // z in the row's unit is 2^100 or more: the unit goes down, weights hardly count beside it
+                    const int high = exponent(__builtin_fabsf(z)), next = high + held > 390 ? 350 - high : held;
+                    const float fo = __builtin_ldexpf(1.0f, next - held);
+                    wsum[cb] *= fo;
 #pragma unroll
-                for (int i = 0; i < NB; i++) o[cb][i] -= wsum[cb];
-                wsum[cb] = v4f{0, 0, 0, 0};
+                    for (int i = 0; i < NB; i++) o[cb][i] *= fo;
+                    one[cb] = power(next), held = next;
+                }
+                const v4f d = __builtin_ldexpf(z, held - 163) - wsum[cb];
+#pragma unroll
+                for (int i = 0; i < NB; i++) o[cb][i] += d;
+                wsum[cb] = v4f{0, 0, 0, 0}, zsum[cb] = 0.0f;
             }
         }
 #pragma unroll

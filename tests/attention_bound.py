@@ -8,8 +8,9 @@ The bound of a result o = sum_t P_t v_t, with u = 2^-24, key k_t = kz + ks code 
   weights   P vs is rounded to float16: 2^-11 of itself, or 2^-22 as the sum of two (float16 results), after two roundings in fp32; what is below
             float16's smallest step is lost: 2^-27 of the row's largest P vs
   sums      over 16 steps of 32 tokens sums of code * weight and of 8 * weight grow to (15 + 8) sum P vs of theirs, half of that in the mean, and each
-            instruction is off by up to 8 u of what it sums (addends aligned, cut off and rounded): 16 * 8 u * 23 / 2 = 64 * 23 u of sum P vs.  What is kept of them
-            is rounded every 16 steps; sums of P and of P vz run through a quarter of the tokens in a lane
+            instruction is off by up to 8 u of what it sums (addends aligned, cut off and rounded): 16 * 8 u * 23 / 2 = 64 * 23 u of sum P vs; the sum of P vz runs
+            through 128 tokens in a lane meanwhile.  What they make together is added to the output so far, at most sum P |v|, by which each of n / 32 steps is off by
+            8 u again; the sum of P runs through a quarter of all tokens in a lane
   result    8 u of it for the quotient, and half a step of its type (below its normal numbers: of the smallest of those)"""
 import math
 
@@ -62,7 +63,7 @@ def bound(cache, table, lens, starts, q, scale=None):
         from_scores = pe @ v.abs() + o.abs() * pe.sum(1, keepdim=True)
         size = w @ vc.abs()
         lost = 2.0 ** -27 * w.amax(1, keepdim=True) * ((~hidden).double() @ vc.abs())
-        sums = 64 * 23 * U * w.sum(1, keepdim=True) + (n / 16 + 2) * U * size + (n / 4 + 64) * U * ((p @ vz.abs())[:, None] + o.abs())
+        sums = 64 * 23 * U * w.sum(1, keepdim=True) + (n / 4 + 2) * U * (p @ v.abs()) + (min(n / 4, 128) + 64) * U * (p @ vz.abs())[:, None] + (n / 4 + 64) * U * o.abs()
         total = from_scores + (unit + 2 * U) * size + lost + sums + o.abs() * (info.eps / 2 + 8 * U) + info.smallest_normal * info.eps / 2
         out[rows], slack[rows] = o.view(shape), total.view(shape)
     return out, slack

@@ -88,18 +88,18 @@ def two_halves(heads, group, dim, page, dtype, sequences=1, seed=4):
     return cache, table, lens, starts, q.to(dtype)
 
 
-def cancelling(heads, group, page, length, sequences, dtype, seed=5):
+def cancelling(heads, group, page, length, sequences, dtype, mean=8, seed=5):
     """every 32 tokens are followed by 32 of the same keys and the opposite values: outputs are 0, whatever the weights.  One long sequence, which all sequences of
-    the call share; values are 1024 (code - 8)"""
+    the call share; values are 1024 (code - mean)"""
     dim = 64
     cache, table, lens, starts, g = make(heads, dim, page, [length], [1], seed)
     at = torch.arange(length) // page, torch.arange(length) % page
     twice = lambda a, b: torch.stack([a, b], 1).view(length, heads, dim)
     keys = torch.randint(0, 16, (length // 64, 32, heads, dim), generator=g, dtype=torch.uint8)
-    side = torch.randint(0, 2, (length // 64, 32, heads, dim), generator=g, dtype=torch.uint8) * 2 + 7
-    cache.k[at[0], :, at[1]], cache.v[at[0], :, at[1]] = twice(keys, keys), twice(side, 16 - side)
+    side = torch.randint(0, 2, (length // 64, 32, heads, dim), generator=g, dtype=torch.uint8) * 2 + mean - 1
+    cache.k[at[0], :, at[1]], cache.v[at[0], :, at[1]] = twice(keys, keys), twice(side, 2 * mean - side)
     cache.kp[..., 0], cache.kp[..., 1] = 0.125, -0.9375
-    cache.vp[..., 0], cache.vp[..., 1] = 1024.0, -8192.0
+    cache.vp[..., 0], cache.vp[..., 1] = 1024.0, -1024.0 * mean
     q = torch.zeros((sequences, heads * group, dim))
     one = torch.randint(0, dim, q.shape[:-1], generator=g)
     q.scatter_(2, one[..., None], (torch.rand(one.shape, generator=g) * 2 - 1)[..., None] * dim ** 0.5)

@@ -75,6 +75,16 @@ def test_sums_do_not_grow_with_the_length(dtype):
     assert float(out.square().mean().sqrt()) <= 272 * 2.0 ** -24 * 1024
 
 
+@pytest.mark.parametrize("mean", [1, 5, 14])
+def test_sums_far_from_the_middle_of_the_codes(mean):
+    """the same with values that cancel about another code than 8, where what codes add and what the tokens' zeros add cancel too.  In 16 steps sums of code * weight
+    and of 8 * weight grow to 15 and 8 times the weights of those steps: 16 * 2 u * (15 + 8) / 2 = 368 u of the weights.  The zeros add 7 times the weights, through 128
+    tokens in a lane: if all adds went one way, 128 u / 2 * 7 / 2 = 224 u.  The weights themselves are float16 twice: 2^-22 of 7 times them, 28 u"""
+    call = cases.cancelling(2, 16383, 64, 131072, 2, torch.float16, mean)
+    out = _run(call).double()
+    assert float(out.square().mean().sqrt()) <= 620 * 2.0 ** -24 * 1024
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads,group,dim,lens,new", [(2, 4, 128, [5, 16, 33, 48, 330, 650], [1] * 6), (1, 8, 64, [1290, 17], [1, 1]), (1, 4, 256, [1001, 500], [3, 2]), (12, 5, 128, [1290], [1050]), (16, 4, 64, [1101], [1000])])
 def test_what_the_table_holds_behind_the_sequences(heads, group, dim, lens, new, dtype):
@@ -119,3 +129,16 @@ def test_values_at_the_ends_of_bfloat16(heads, group, dim, page, length, new, ex
     call = cases.mixed(heads, group, dim, page, [length], [new], 6, torch.bfloat16)
     call[0].vp *= 2.0 ** exponent
     _check(call)
+
+
+@pytest.mark.parametrize("some", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,group,dim,page,length,new", [(1, 4, 64, 16, 9000, 1), (2, 4, 128, 64, 5000, 2), (1, 2, 256, 16, 5000, 3), (16, 4, 64, 32, 1700, 1000), (12, 5, 128, 64, 1700, 1050)])
+def test_values_that_are_all_alike_in_a_token(heads, group, dim, page, length, new, dtype, some):
+    """scales of 0 beside zeros that are not, over more than one run of 16 steps; `some`: tokens of ordinary values among them, small ones"""
+    cache, table, lens, starts, g = cases.make(heads, dim, page, [length], [new], 7)
+    alike = torch.rand(cache.vp.shape[:-1], generator=g) < (0.9 if some else 2)
+    cache.vp *= 2.0 ** -10
+    cache.vp[..., 0].masked_fill_(alike, 0.0)
+    cache.vp[..., 1] = torch.where(alike, torch.randn(alike.shape, generator=g) * (1e4 if dtype == "f16" else 1e32), cache.vp[..., 1].float()).bfloat16()
+    _check((cache, table, lens, starts, cases.queries(cache, starts, group, TYPES[dtype], g)))
