@@ -403,7 +403,7 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4 kv, T* K, T* V) {
 // third are joined to the first, which so holds outputs, and no other sum goes over more than 512 tokens (131072 tokens whose values cancel, about code 8 / about code 1:
 // off by 3e-5 / 5e-4 of the weights with each sum by itself, now 1e-7 / 2e-6, for 4 % of a prompt's time; -8 as one more operand of each
 // block of channels, so that no sum grows at all, costs 12 to 19 %).  Queries are scaled by a power of two so that their largest
-// magnitude is in [2^14, 2^15): a float16 or bfloat16 keeps all of its bits, down to 2^-38 of the largest.  Weights have a unit of their own in
+// magnitude is in [2^14, 2^15): a float16 or bfloat16 keeps all of its bits, down to 2^-34 of the largest (2^-38 where codes do not count 16 times).  Weights have a unit of their own in
 // each row, a power of two that follows the largest p vs that the row has met (not the largest vs: a token that the row does not see, or hardly, does not move it): that
 // one is 2^6 or more, at most 2^15, and what is below 2^-27 of it is lost.  What weights are relative to is a power of two as well, so
 // that both move without a rounding.
@@ -681,6 +681,25 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT, D * CB <= 256 && D < 256 ?
         }
         __builtin_amdgcn_sched_barrier(0);
         keys_done();
+        if ((t0 / (32 * WT)) % 16 == 0) {
+#pragma unroll
+            for (int cb = 0; cb < CB; cb++) {
+                const float z = sum_over_quarters(zsum[cb]);
+                int held = exponent(one[cb]);
+                if (__any(exponent(__builtin_fabsf(z)) + held > 390)) {   // z in the row's unit is 2^100 or more: the unit goes down, weights hardly count beside it
+                    const int high = exponent(__builtin_fabsf(z)), next = high + held > 390 ? 350 - high : held;
+                    const float fo = __builtin_ldexpf(1.0f, next - held);
+                    wsum[cb] *= fo;
+#pragma unroll
+                    for (int i = 0; i < NB; i++) o[cb][i] *= fo;
+                    one[cb] = power(next), held = next;
+                }
+                const v4f d = __builtin_ldexpf(z, held - 163) - wsum[cb];
+#pragma unroll
+                for (int i = 0; i < NB; i++) o[cb][i] += d;
+                wsum[cb] = v4f{0, 0, 0, 0}, zsum[cb] = 0.0f;
+            }
+        }
         v8h wh[CB], wl[PARTS == 2 ? CB : 1];
 #pragma unroll
         for (int cb = 0; cb < CB; cb++) {
@@ -741,25 +760,6 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT, D * CB <= 256 && D < 256 ?
             if (PARTS == 2) wl[PARTS == 2 ? cb : 0] = __builtin_bit_cast(v8h, (v4u{lo[0], lo[1], lo[2], lo[3]}));
         }
         __builtin_amdgcn_sched_barrier(0);
-        if ((t0 / (32 * WT)) % 16 == 0) {
-#pragma unroll
-            for (int cb = 0; cb < CB; cb++) {
-                const float z = sum_over_quarters(zsum[cb]);
-                int held = exponent(one[cb]);
-                if (__any(exponent(__builtin_fabsf(z)) + held > 390)) {   // z in the row's unit is 2^100 or more: the unit goes down, weights hardly count beside it
-                    const int high = exponent(__builtin_fabsf(z)), next = high + held > 390 ? 350 - high : held;
-                    const float fo = __builtin_ldexpf(1.0f, next - held);
-                    wsum[cb] *= fo;
-#pragma unroll
-                    for (int i = 0; i < NB; i++) o[cb][i] *= fo;
-                    one[cb] = power(next), held = next;
-                }
-                const v4f d = __builtin_ldexpf(z, held - 163) - wsum[cb];
-#pragma unroll
-                for (int i = 0; i < NB; i++) o[cb][i] += d;
-                wsum[cb] = v4f{0, 0, 0, 0}, zsum[cb] = 0.0f;
-            }
-        }
 #pragma unroll
         for (int i = 0; i <= NB; i++) {
             const v8h a = i == NB ? __builtin_bit_cast(v8h, eights) : codes8(x.vw[i == NB ? 0 : i]);
