@@ -186,7 +186,7 @@ __device__ __forceinline__ void unpack32(uint32_t s, uint32_t z, uint32_t (&out)
 // Few tokens: KS wavefronts split K over one tile of 16 NB weight rows x 16 MB tokens and meet in LDS.  Operands come straight from memory
 // into registers, the next step's while this one is multiplied.  What a compute unit can have on its way through its L1 bounds codes (17 bytes per clock; two,
 // three or four steps ahead are no faster than one), 1 x 4096 x 4096 6.1 us with its launch; packed weights are bounded by memory for one token (16384 x 16384
-// ternary 17.6 us, 3.8 TB/s, from HBM) and by unpacking, 4 instructions per word of codes, for many.
+// ternary 17.6 us, 3.8 TB/s, from HBM; binary 12.6) and by unpacking, 4 instructions per word of codes, for many.
 template <I8Weights W, typename T, int NB, int MB, bool TOKENS>
 __global__ __launch_bounds__(512) void k_i8_few(I8Product p, uint32_t ntiles) {
     constexpr int KS = 8, LD = 16 * NB + 4;

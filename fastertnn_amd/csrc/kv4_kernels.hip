@@ -247,9 +247,9 @@ __device__ __forceinline__ void group_range(const float (&y)[8], bool live, floa
 }
 
 // A wavefront per (block of 8 positions, head of keys and values, or behind those of queries); where there are many it takes one head after the other, so
-// that finding the block is paid once for several.  Memory bounds it at first, then the chain of loads (starts, table, rows) of few
-// wavefronts: the angles' 64-bit products take registers.  5 x 4001 new tokens, 8 heads of 64 with 16 of queries: 38 us for 140 MB (3.7 TB/s); 48 x 1
-// of 8 + 32 heads of 128: 5 us on the device.  LG lanes hold a token's channels, eight each.  The codes of a block's values meet in LDS, where every lane makes the words of its channels; what the block holds already of
+// that finding the block is paid once for several.  Of many tokens the vector ALU bounds it, with the angles' 64-bit products and the codes (busy 76 % of the
+// launch): 5 x 4001 new tokens, 8 heads of 64 with 16 of queries: 35 us for 108 MB (3.1 TB/s).  Of few it is the chain of loads (starts, table, rows): 48 x 1
+// of 8 + 32 heads of 128: 7 us on the device, where an empty launch is 2.4.  LG lanes hold a token's channels, eight each.  The codes of a block's values meet in LDS, where every lane makes the words of its channels; what the block holds already of
 // other tokens stays.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_kv4_append(Kv4 kv, Kv4Rows k, Kv4Rows v, Kv4Rotation r, int heads_q, Kv4Rows q, T* q_out) {
@@ -350,7 +350,7 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4 kv, Kv4Rows k, Kv4Rows v
 }
 
 // The same blocks and lanes the other way round: a lane's eight channels of a token are one word of keys, and eight words that hold its token among others,
-// which the block's other lanes find in the L1.  Stores bound it: the tokens above in 10 us, 41 MB of results.
+// which the block's other lanes find in the L1.  Stores bound it: the tokens above in 11 us, 33 MB of results.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_kv4_read(Kv4 kv, T* K, T* V) {
     constexpr int LG = D <= 64 ? 8 : D <= 128 ? 16 : 32, TPI = 64 / LG;
@@ -412,9 +412,9 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4 kv, T* K, T* V) {
 // lane quarter g ends with the scores of tokens 8 g .. 8 g + 7 of its column (a query), in the order in which the second product takes
 // its weights as B operand: no lanes are exchanged.  The values of 8 tokens of a channel are one word of the cache, its A operand.
 //
-// What bounds it: of one token per sequence the cache's bytes (65003 tokens of 8 x 4 heads of 128: 22 us, 3.2 TB/s with two launches; 64 sequences of 4000
-// 4.2 TB/s), with 8 heads of 64 per head of keys the vector ALU; of prompts the vector ALU, at 14 instructions per score of a wavefront beside the matrix
-// instructions (2 x 2500 new of 4099, 8 x 4 heads of 128: 367 us, 0.5 PFLOP/s).
+// What bounds it: of one token per sequence the cache's bytes (65003 tokens of 8 x 4 heads of 128: 21.3 us, 3.3 TB/s with two launches; 64 sequences of 2000 to
+// 4000 43.5 us, 4.8 TB/s), with 8 heads of 64 per head of keys the vector ALU; of prompts the vector ALU, at 24 instructions per score of a wavefront beside two matrix
+// instructions (2 x 2500 new of 4099, 8 x 4 heads of 128: 356 us, 0.5 PFLOP/s).
 // Rows of a tile are (token, query head of the group) pairs of one sequence and one head of keys.
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));

@@ -163,7 +163,7 @@ PyObject* net_run(PyObject*, PyObject* const* v, Py_ssize_t n) {
 }
 
 // ---- operators of token models.  These make the results that they are not given, and return them: a product of one token
-// takes 13.0 us through ctypes, 5.5 here, of which the launch is 4.  What does not have the plain form that a wrapper asks for is left to the wrapper, which says why.
+// takes 15.8 us through ctypes, 5.6 here, of which the launch is 4.  What does not have the plain form that a wrapper asks for is left to the wrapper, which says why.
 
 struct Tensors {
     bool good = true;

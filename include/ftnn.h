@@ -459,7 +459,7 @@ FTNN_API int ftnn_kv4_read(const ftnn_kv4_t *kv, int dtype, void *d_k, void *d_v
  * contiguous, of the queries' type (FTNN_F16 or FTNN_BF16); zeros for a query that sees no token.  max_len: the largest of lens if the
  * caller knows it, else 0; it decides how the work is split and nothing else.  d_scratch: 16-byte aligned,
  * ftnn_kv4_attention_scratch_bytes() bytes (0: none needed).  Products are computed in float16 with fp32 sums, the
- * weights of FTNN_F16 as two float16 each.
+ * weights of FTNN_F16 as two float16 each, in units of the largest weight * scale of their row: what is below 2^-27 of that is lost.
  */
 FTNN_API int64_t ftnn_kv4_attention_scratch_bytes(const ftnn_kv4_t *kv, int heads_q, int max_len);
 FTNN_API int ftnn_kv4_attention(const ftnn_kv4_t *kv, int dtype, int heads_q, const void *d_q, int64_t q_token_stride,
